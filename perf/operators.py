@@ -5,8 +5,9 @@
 ``run(state)`` is one pass and ``work(case)`` what a pass cannot do without.
 With ``own`` false the operators are computed in plain form: elementary torch
 operations in 32 bits, each output rounded once.  With ``own`` true ``run``
-calls ``bayes_ssm.causal_conv``, ``causal_conv_step``, ``selective_scan``,
-``selective_step`` and ``distillation_loss``.  ``exact(case, seed)`` computes
+calls ``causal_conv``, ``causal_conv_step``, ``selective_scan`` and
+``selective_step`` of ``bayes_ssm.selective`` and
+``bayes_ssm.distill.distillation_loss``.  ``exact(case, seed)`` computes
 the same outputs in 64 bits by other means.
 
 The operators, per sequence and channel:
@@ -37,8 +38,8 @@ def _package():
     root = str(Path(__file__).resolve().parents[1] / "bayes-ssm_b200")
     if root not in sys.path:
         sys.path.insert(0, root)
-    import bayes_ssm
-    return bayes_ssm
+    from bayes_ssm import distill, selective
+    return selective, distill
 
 
 # ---------------------------------------------------------------------------
@@ -259,7 +260,7 @@ def prepare(case, seed):
         leaves = ("logits",)
     if own:
         if case.get("packed"):
-            st["sequences"] = _package().PackedSequences(_lengths(case), device="cuda")
+            st["sequences"] = _package()[0].PackedSequences(_lengths(case), device="cuda")
         if op == "distill" or case["train"]:
             st["leaves"] = [k for k in leaves if st[k] is not None]
             for k in st["leaves"]:
@@ -275,26 +276,26 @@ def prepare(case, seed):
 
 def _own(st):
     case = st["case"]
-    bayes_ssm = _package()
+    selective, distill = _package()
     op = case["op"]
     if op == "conv_step":
-        y = bayes_ssm.causal_conv_step(st["x"], st["state"], st["weight"], st["bias"],
+        y = selective.causal_conv_step(st["x"], st["state"], st["weight"], st["bias"],
                                        activation="silu" if case["silu"] else None)
         return y, st["state"]
     if op == "step":
-        y = bayes_ssm.selective_step(st["values"], st["steps"], st["rates"], st["keys"], st["queries"], st["state"],
+        y = selective.selective_step(st["values"], st["steps"], st["rates"], st["keys"], st["queries"], st["state"],
                                      skip=st["skip"], gate=st["gate"], step_bias=st["step_bias"], softplus=True)
         return y, st["state"]
     if op == "distill":
-        loss = bayes_ssm.distillation_loss(st["logits"], st["teacher"], st["indices"],
+        loss = distill.distillation_loss(st["logits"], st["teacher"], st["indices"],
                                            temperature=case["temperature"])
         return loss, torch.autograd.grad(loss, st["logits"])[0]
     if op == "conv":
-        out = bayes_ssm.causal_conv(st["x"], st["weight"], st["bias"], activation="silu" if case["silu"] else None,
+        out = selective.causal_conv(st["x"], st["weight"], st["bias"], activation="silu" if case["silu"] else None,
                                     initial_state=st["state"], sequences=st.get("sequences"))
         upstream = [st.get("grad"), None]
     else:
-        out = bayes_ssm.selective_scan(st["values"], st["steps"], st["rates"], st["keys"], st["queries"],
+        out = selective.selective_scan(st["values"], st["steps"], st["rates"], st["keys"], st["queries"],
                                        skip=st["skip"], gate=st["gate"], step_bias=st["step_bias"], softplus=True,
                                        initial_state=st["state"], sequences=st.get("sequences"))
         upstream = [st.get("grad"), st.get("grad_state")]
