@@ -63,6 +63,23 @@ _SIGNATURES = {
     "bssm_rotation_backward_chunked": ([_i, _i, _i] + [_vp] * 22 + [_sz, _l, _l, _i, _d, _vp], _i),
     "bssm_rotation_coefficients": ([_vp, _vp, _l, _vp, _vp, _vp], _i),
     "bssm_rotation_coefficients_backward": ([_vp, _vp, _vp, _vp, _l, _vp, _vp, _vp], _i),
+    "bssm_causal_conv": ([_vp, _i, _l, _l, _i, _i, _vp, _i, _vp, _i, _i, _vp, _l, _vp, _vp, _vp, _vp], _i),
+    "bssm_causal_conv_partial_floats": ([_l, _i, _i], _l),
+    "bssm_causal_conv_backward": ([_vp, _i, _l, _l, _i, _i, _vp, _i, _vp, _i, _i, _vp, _l] + [_vp] * 8
+                                  + [_l, _vp], _i),
+    "bssm_causal_conv_step": ([_vp, _i, _l, _l, _i, _i, _vp, _i, _vp, _i, _i, _vp, _vp, _vp], _i),
+    "bssm_selective_saved_floats": ([_l, _l, _i, _i], _l),
+    "bssm_selective_scan": ([_vp, _l] * 5 + [_i, _vp, _vp, _vp, _i, _l, _i, _i, _i, _vp, _l, _vp, _vp, _vp, _vp, _l,
+                                             _vp], _i),
+    "bssm_selective_backward_floats": ([_l, _l, _i, _i, _i], _l),
+    "bssm_selective_scan_backward": ([_vp, _l] * 5 + [_i, _vp, _vp, _vp, _i, _l, _i, _i, _i, _vp, _l] + [_vp] * 13
+                                     + [_l, _vp], _i),
+    "bssm_selective_step": ([_vp, _l] * 5 + [_i, _vp, _vp, _vp, _i, _l, _i, _i, _i, _vp, _vp, _vp], _i),
+    "bssm_distillation": ([_vp, _i, _l, _i, _l, _vp, _i, _vp, _i, _i, ctypes.c_float, _i, _vp, _vp, _vp, _vp, _vp,
+                           _vp], _i),
+    "bssm_distillation_backward": ([_vp, _i, _l, _i, _l, _vp, _i, _vp, _i, _i, ctypes.c_float, _i, _vp, _vp, _vp, _i,
+                                    _vp, _vp], _i),
+    "bssm_distillation_scale": ([_vp, _i, _l, _vp, _vp], _i),
     "bssm_debug_wait_timeouts": ([], ctypes.c_uint),
     "bssm_stream_status": ([_vp], _i),
     "bssm_debug_wait_probe": ([_i, _vp], _i),

@@ -1,0 +1,151 @@
+"""Distillation from a teacher's top logits.
+
+Per row, with ``p`` the teacher's softmax over the ``K`` logits it gives and
+``q`` the student's over the whole vocabulary, both at a temperature:
+``loss = temperature^2 * sum_k p_k (log p_k - log q_{i_k})``.
+
+On CUDA one sm_100a kernel per row (``csrc/bssm_distill.cu``) reads the logits
+and, where the loss is reduced to one number, writes their gradient in the same
+launch, so a training step reads the logits once and writes the gradient once;
+on CPU the formula runs as PyTorch operations.
+"""
+from __future__ import annotations
+
+import math
+from numbers import Real
+
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from . import _capi
+from .selective import _DTYPES, _gradients_wanted, _rows, _stream
+
+MAX_TOP = 1024
+
+
+def distillation_loss_torch(logits: Tensor, teacher_logits: Tensor, teacher_indices: Tensor, *,
+                            temperature: float = 1.0, reduction: str = "mean") -> Tensor:
+    """:func:`distillation_loss` in PyTorch operations, computed in float32
+    (float64 for float64 logits)."""
+    wide = torch.promote_types(logits.dtype, torch.float32)
+    live = (teacher_indices >= 0) & (teacher_logits != -math.inf)
+    counted = live.any(-1)
+    t = torch.where(live, teacher_logits.to(wide) / temperature, -math.inf)
+    t = torch.where(counted[..., None], t, 0.0)
+    log_p = torch.log_softmax(t, -1)
+    p = torch.where(live, torch.exp(log_p), 0.0)
+    bad = (live & (teacher_indices >= logits.shape[-1])).any(-1)
+    index = teacher_indices.long().clamp(0, logits.shape[-1] - 1)
+    s = torch.where((counted & ~bad)[..., None], logits.to(wide), 0.0)
+    log_q = torch.gather(torch.log_softmax(s / temperature, -1), -1, index)
+    # an entry of no weight adds nothing, whatever its logarithms
+    term = torch.where(p != 0, p * (log_p - torch.where(p != 0, log_q, 0.0)), 0.0)
+    rows = torch.where(counted, term.sum(-1) * temperature * temperature, 0.0)
+    rows = torch.where(bad, math.nan, rows)
+    if reduction == "none":
+        return rows
+    total = rows.sum()
+    return total / counted.sum().clamp(min=1) if reduction == "mean" else total
+
+
+class _Distillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, teacher, indices, temperature, reduction, with_grad):
+        dev = logits.device
+        vocab, top = logits.shape[-1], teacher.shape[-1]
+        rows = teacher.numel() // top
+        x, stride = _rows(logits, 1)
+        teacher, indices = teacher.contiguous(), indices.contiguous()
+        mean, reduced = int(reduction == "mean"), reduction != "none"
+        stats = torch.empty(rows, 2, device=dev, dtype=torch.float32)
+        row_loss = torch.empty(logits.shape[:-1], device=dev, dtype=torch.float32)
+        loss = torch.empty((), device=dev, dtype=torch.float32) if reduced else None
+        count = torch.empty(1, device=dev, dtype=torch.int32)
+        # one number: its gradient is known here up to a factor
+        grad = torch.empty(logits.shape, device=dev, dtype=logits.dtype) if with_grad and reduced else None
+        with torch.cuda.device(dev):
+            rc = _capi.load().bssm_distillation(
+                x.data_ptr(), _DTYPES[x.dtype], rows, vocab, stride, teacher.data_ptr(), _DTYPES[teacher.dtype],
+                indices.data_ptr(), indices.element_size(), top, temperature, mean, row_loss.data_ptr(),
+                stats.data_ptr(), _capi.ptr(loss), count.data_ptr(), _capi.ptr(grad), _stream(dev))
+        _capi.check(rc, "bssm_distillation")
+        if with_grad:
+            ctx.save_for_backward(logits, teacher, indices, stats, count)
+            ctx.settings = (temperature, mean, reduced)
+            ctx.grad = grad
+        return loss if reduced else row_loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, upstream):
+        logits, teacher, indices, stats, count = ctx.saved_tensors
+        temperature, mean, reduced = ctx.settings
+        dev = logits.device
+        upstream = upstream.float().contiguous()
+        # The gradient written by the forward is handed out once, times the
+        # upstream one; a second walk through a retained graph makes its own.
+        grad, ctx.grad = ctx.grad, None
+        with torch.cuda.device(dev):
+            lib = _capi.load()
+            if grad is not None:
+                rc = lib.bssm_distillation_scale(grad.data_ptr(), _DTYPES[grad.dtype], grad.numel(),
+                                                 upstream.data_ptr(), _stream(dev))
+                _capi.check(rc, "bssm_distillation_scale")
+            else:
+                x, stride = _rows(logits, 1)
+                top = teacher.shape[-1]
+                grad = torch.empty(logits.shape, device=dev, dtype=logits.dtype)
+                rc = lib.bssm_distillation_backward(
+                    x.data_ptr(), _DTYPES[x.dtype], teacher.numel() // top, logits.shape[-1], stride,
+                    teacher.data_ptr(), _DTYPES[teacher.dtype], indices.data_ptr(), indices.element_size(), top,
+                    temperature, mean, stats.data_ptr(), count.data_ptr(), upstream.data_ptr(), int(not reduced),
+                    grad.data_ptr(), _stream(dev))
+                _capi.check(rc, "bssm_distillation_backward")
+        return grad, None, None, None, None, None
+
+
+def distillation_loss(logits: Tensor, teacher_logits: Tensor, teacher_indices: Tensor, *, temperature: float = 1.0,
+                      reduction: str = "mean") -> Tensor:
+    """``temperature^2 * KL(teacher || student)`` over a teacher's top logits.
+
+    ``logits`` are the student's ``[..., V]``; ``teacher_logits [..., K]`` the
+    teacher's logits at vocabulary entries ``teacher_indices [..., K]`` (int32
+    or int64).  An entry with a negative index or a logit of ``-inf`` is empty;
+    a row of empty entries (a prompt's, or padding) has loss and gradient zero
+    and does not count in a mean.  An index at or past V makes the row's loss
+    and gradient NaN.  ``reduction`` is ``"mean"`` (over the rows that count;
+    zero if none does), ``"sum"`` or ``"none"`` (``[...]``).  The loss is
+    float32; gradients flow to ``logits`` only.  CUDA takes up to 1,024 teacher
+    logits a row.
+    """
+    if logits.ndim < 1 or teacher_logits.ndim != logits.ndim or teacher_logits.shape[:-1] != logits.shape[:-1]:
+        raise ValueError("teacher_logits must be [..., K] with the logits' leading dimensions")
+    if teacher_indices.shape != teacher_logits.shape:
+        raise ValueError("teacher_indices must have the teacher_logits' shape")
+    if logits.shape[-1] < 1 or teacher_logits.shape[-1] < 1:
+        raise ValueError("logits and teacher_logits must not be empty")
+    if not logits.is_floating_point() or not teacher_logits.is_floating_point():
+        raise TypeError("logits and teacher_logits must have floating-point dtype")
+    if teacher_indices.dtype not in (torch.int32, torch.int64):
+        raise TypeError("teacher_indices must be int32 or int64")
+    if teacher_logits.device != logits.device or teacher_indices.device != logits.device:
+        raise ValueError("logits, teacher_logits and teacher_indices must be on the same device")
+    if isinstance(temperature, bool) or not isinstance(temperature, Real) or not math.isfinite(temperature) \
+            or temperature <= 0:
+        raise ValueError("temperature must be finite and positive")
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError("reduction must be 'mean', 'sum' or 'none'")
+    if not logits.is_cuda:
+        return distillation_loss_torch(logits, teacher_logits.detach(), teacher_indices, temperature=temperature,
+                                       reduction=reduction)
+    if logits.dtype not in _DTYPES or teacher_logits.dtype not in _DTYPES:
+        raise TypeError("distillation_loss on CUDA takes float32, bfloat16 or float16 logits")
+    if teacher_logits.shape[-1] > MAX_TOP:
+        raise NotImplementedError(f"distillation_loss on CUDA needs at most {MAX_TOP} teacher logits a row "
+                                  f"(got {teacher_logits.shape[-1]}); use distillation_loss_torch")
+    return _Distillation.apply(logits, teacher_logits.detach(), teacher_indices, float(temperature), reduction,
+                               _gradients_wanted(logits))
+
+
+__all__ = ["distillation_loss", "distillation_loss_torch"]

@@ -1,0 +1,90 @@
+// bssm_io.cuh -- element types and packed sequences of the operators that take
+// float32, bfloat16 and float16 rows (causal convolution, selective scan,
+// distillation).  Everything is widened to float32 on load and rounded once on
+// store.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "bayes_ssm_b200.h"
+
+namespace bssm {
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+
+template <typename T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+
+// Elements of parameters (weights, biases) keep their own type: element i of
+// an array whose type is a BSSM_* code.
+__device__ __forceinline__ float load_as_float(const void *p, int dtype, long i) {
+    if (dtype == BSSM_F32) return static_cast<const float *>(p)[i];
+    if (dtype == BSSM_BF16) return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+    return __half2float(static_cast<const __half *>(p)[i]);
+}
+__device__ __forceinline__ void store_from_float(void *p, int dtype, long i, float v) {
+    if (dtype == BSSM_F32) static_cast<float *>(p)[i] = v;
+    else if (dtype == BSSM_BF16) static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(v);
+    else static_cast<__half *>(p)[i] = __float2half_rn(v);
+}
+
+__host__ __device__ constexpr bool io_dtype_known(int dtype) {
+    return dtype == BSSM_F32 || dtype == BSSM_BF16 || dtype == BSSM_F16;
+}
+__host__ __device__ constexpr int io_dtype_bytes(int dtype) { return dtype == BSSM_F32 ? 4 : 2; }
+
+// VEC consecutive elements as float32, in one access when VEC * sizeof(T) <= 16
+// (the address must then be a multiple of that), else in 16-byte accesses.
+template <typename T, int VEC> struct alignas(VEC * sizeof(T) < 16 ? VEC * sizeof(T) : 16) Packed {
+    T e[VEC];
+};
+template <typename T, int VEC> __device__ __forceinline__ void widen(const Packed<T, VEC> &p, float (&o)[VEC]) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) o[i] = to_float(p.e[i]);
+}
+template <typename T, int VEC> __device__ __forceinline__ Packed<T, VEC> load_packed(const T *p) {
+    return *reinterpret_cast<const Packed<T, VEC> *>(p);
+}
+template <typename T, int VEC> __device__ __forceinline__ void store_packed(T *p, const float (&v)[VEC]) {
+    Packed<T, VEC> o;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) o.e[i] = from_float<T>(v[i]);
+    *reinterpret_cast<Packed<T, VEC> *>(p) = o;
+}
+
+__device__ __forceinline__ float sigmoid_f(float x) { return 1.f / (1.f + __expf(-x)); }
+
+// The sequences in the token rows: `count` runs of `length` tokens each, or,
+// with offsets (count + 1 int64 values from 0 to tokens, never decreasing),
+// run s from offsets[s] to offsets[s + 1].  Bounds are clamped to the rows
+// there are, so offsets outside the contract read nothing out of range.
+struct Sequences {
+    const long *offsets;
+    long count, length, tokens;
+
+    __device__ __forceinline__ long begin(long s) const {
+        if (offsets == nullptr) return s * length;
+        const long o = offsets[s];
+        return o < 0 ? 0 : (o > tokens ? tokens : o);
+    }
+    __device__ __forceinline__ long end(long s) const { return offsets == nullptr ? (s + 1) * length : begin(s + 1); }
+    // The sequence that holds token row g (g < tokens).
+    __device__ __forceinline__ long find(long g) const {
+        if (offsets == nullptr) return g / length;
+        long lo = 0, hi = count;  // offsets[lo] <= g < offsets[hi]
+        while (hi - lo > 1) {
+            const long mid = (lo + hi) / 2;
+            if (offsets[mid] <= g) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    }
+};
+
+}  // namespace bssm

@@ -48,7 +48,7 @@ extern "C" {
 
 #define BSSM_F32 0
 #define BSSM_BF16 1
-#define BSSM_F16 2 /* bssm_check_values only */
+#define BSSM_F16 2 /* bssm_check_values, the selective operators and distillation */
 
 /* Message for the last failing call on this thread ("" after success). */
 const char *bssm_last_error(void);
@@ -418,6 +418,104 @@ int bssm_envelope_epilogue_backward(const void *read, int read_dtype, const void
                                     int heads, int head_dim, const void *grad_out, void *grad_read, void *grad_gate,
                                     long grad_gate_row_stride, float *grad_norm_weight, float *workspace,
                                     long workspace_floats, void *stream);
+
+/*
+ * Operators of a selective state space layer (no counterpart in the reference).
+ *
+ * Token rows: `tokens` rows hold `sequences` sequences, of one length each
+ * (offsets null, tokens divisible by sequences) or packed one after the other
+ * (offsets: sequences + 1 int64 device values from 0 to tokens, never
+ * decreasing).  Row operands have unit channel stride and rows *_stride
+ * elements apart; outputs and gradients are contiguous.  dtype (BSSM_F32,
+ * BSSM_BF16 or BSSM_F16) is that of the rows; sums and states of the scan are
+ * float32.  Sums over tokens or channels are taken in a fixed order.
+ *
+ * bssm_causal_conv: y_t = act(bias + sum_j w_j x_{t-taps+1+j}) per channel,
+ * act the identity or (silu != 0) SiLU; taps is 2, 3 or 4.  weight [channels]
+ * [taps] and bias [channels] (may be null) have their own dtypes.  state0
+ * (null: zeros) and state1 (null: not written) [sequences][taps-1][channels]
+ * hold the inputs before the first and after the last token, oldest first, in
+ * the rows' dtype.
+ * bssm_causal_conv_backward: grad_state1 null is zero; grad_bias and
+ * grad_state0 may be null.  workspace holds bssm_causal_conv_partial_floats()
+ * floats.
+ * bssm_causal_conv_step: one token per sequence, `state` moved on in place.
+ */
+int bssm_causal_conv(const void *x, int dtype, long row_stride, long tokens, int channels, int taps,
+                     const void *weight, int weight_dtype, const void *bias, int bias_dtype, int silu,
+                     const long *offsets, long sequences, const void *state0, void *y, void *state1, void *stream);
+long bssm_causal_conv_partial_floats(long tokens, int channels, int taps);
+int bssm_causal_conv_backward(const void *x, int dtype, long row_stride, long tokens, int channels, int taps,
+                              const void *weight, int weight_dtype, const void *bias, int bias_dtype, int silu,
+                              const long *offsets, long sequences, const void *state0, const void *grad_y,
+                              const void *grad_state1, void *grad_x, void *grad_weight, void *grad_bias,
+                              void *grad_state0, float *workspace, long workspace_floats, void *stream);
+int bssm_causal_conv_step(const void *x, int dtype, long row_stride, long sequences, int channels, int taps,
+                          const void *weight, int weight_dtype, const void *bias, int bias_dtype, int silu,
+                          void *state, void *y, void *stream);
+
+/*
+ * bssm_selective_scan: with d = softplus(steps + step_bias) (softplus == 0:
+ * the sum itself), h_t = exp(d_t rates) h_{t-1} + d_t values_t keys_t and
+ * out_t = (queries_t . h_t + skip values_t) SiLU(gate_t), per channel with
+ * `states` (1..64) values of state.  values, steps and gate (may be null) are
+ * [tokens][channels]; keys and queries [tokens][groups][states], a group's
+ * shared by channels / groups adjacent channels; rates [channels][states],
+ * skip and step_bias [channels] (may be null) float32; state0 (null: zeros)
+ * and state1 [sequences][channels][states] float32, state1 16-byte aligned.
+ * saved (16-byte aligned, bssm_selective_saved_floats() floats; null where no
+ * backward follows) receives the states the backward starts its replays from;
+ * its layout is internal.
+ * bssm_selective_scan_backward: grad_out and grad_state1 may be null (zero);
+ * grad_skip, grad_step_bias and grad_state0 may be null (not written).
+ * workspace (16-byte aligned): bssm_selective_backward_floats() floats.
+ * bssm_selective_step: one token per sequence, `state` (16-byte aligned) moved
+ * on in place.
+ */
+long bssm_selective_saved_floats(long tokens, long sequences, int channels, int states);
+int bssm_selective_scan(const void *values, long value_stride, const void *steps, long step_stride, const void *keys,
+                        long key_stride, const void *queries, long query_stride, const void *gate, long gate_stride,
+                        int dtype, const float *rates, const float *skip, const float *step_bias, int softplus,
+                        long tokens, int channels, int states, int groups, const long *offsets, long sequences,
+                        const float *state0, void *out, float *state1, float *saved, long saved_floats, void *stream);
+long bssm_selective_backward_floats(long tokens, long sequences, int channels, int states, int groups);
+int bssm_selective_scan_backward(
+    const void *values, long value_stride, const void *steps, long step_stride, const void *keys, long key_stride,
+    const void *queries, long query_stride, const void *gate, long gate_stride, int dtype, const float *rates,
+    const float *skip, const float *step_bias, int softplus, long tokens, int channels, int states, int groups,
+    const long *offsets, long sequences, const float *saved, const void *grad_out, const float *grad_state1,
+    void *grad_values, void *grad_steps, float *grad_rates, void *grad_keys, void *grad_queries, float *grad_skip,
+    void *grad_gate, float *grad_step_bias, float *grad_state0, float *workspace, long workspace_floats, void *stream);
+int bssm_selective_step(const void *values, long value_stride, const void *steps, long step_stride, const void *keys,
+                        long key_stride, const void *queries, long query_stride, const void *gate, long gate_stride,
+                        int dtype, const float *rates, const float *skip, const float *step_bias, int softplus,
+                        long sequences, int channels, int states, int groups, float *state, void *out, void *stream);
+
+/*
+ * Distillation from a teacher's top logits (no counterpart in the reference).
+ *
+ * Per row, with p the softmax of teacher / temperature over its `top` (1 to
+ * 1,024) logits and q that of logits / temperature over `vocab`:
+ * row_loss = temperature^2 sum_k p_k (log p_k - log q_{i_k}).  An index below
+ * zero or a teacher logit of -inf is an empty entry; a row of empty entries
+ * has loss and gradient zero; an index at or past vocab makes the row's loss
+ * and gradient NaN.  logits rows are row_stride elements apart; teacher and
+ * indices (index_bytes 4 or 8) are [rows][top].
+ * row_stats (two floats a row) is what the backward needs.  loss (may be
+ * null) receives the sum of row_loss, divided, with mean != 0, by the number
+ * of rows that have a teacher, which is left in *count.  grad (may be null)
+ * [rows][vocab] receives the gradient of that loss; the backward writes it
+ * times *upstream, or times upstream[row].
+ * bssm_distillation_scale multiplies n values by the device float *factor.
+ */
+int bssm_distillation(const void *logits, int dtype, long rows, int vocab, long row_stride, const void *teacher,
+                      int teacher_dtype, const void *indices, int index_bytes, int top, float temperature, int mean,
+                      float *row_loss, float *row_stats, float *loss, int *count, void *grad, void *stream);
+int bssm_distillation_backward(const void *logits, int dtype, long rows, int vocab, long row_stride,
+                               const void *teacher, int teacher_dtype, const void *indices, int index_bytes, int top,
+                               float temperature, int mean, const float *row_stats, const int *count,
+                               const float *upstream, int upstream_per_row, void *grad, void *stream);
+int bssm_distillation_scale(void *grad, int dtype, long n, const float *factor, void *stream);
 
 /*
  * Device status (no counterpart in the reference: its kernels have no waits).

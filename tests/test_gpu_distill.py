@@ -1,0 +1,224 @@
+"""GPU: distillation kernels vs the plain 64-bit form.
+
+Tolerances: a float32 logit's exponent (at most about 40 in magnitude here) is
+rounded to 2^-24 of itself and exp2 to 2 ulp, so a probability is good to 40 *
+2^-24 + 2^-22 = 2.6e-6 and the loss and gradient, sums and differences of
+them, to 1e-5 in relative L2; a gradient rounded to bfloat16 (float16) is off
+by at most 2^-9 (2^-12) of itself: 2.5e-3, and 6e-4 plus float16's subnormal
+spacing.
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import plain_selective as plain
+from bayes_ssm.distill import distillation_loss, distillation_loss_torch
+
+pytestmark = pytest.mark.gpu
+
+TOL = {torch.float32: 1e-5, torch.bfloat16: 2.5e-3, torch.float16: 1e-3}
+
+
+def rel(a, b):
+    a, b = a.detach().double(), b.detach().double()
+    return float((a - b).norm() / b.norm().clamp_min(1e-30))
+
+
+def inputs(rows, vocab, top, dtype, seed, index_dtype=torch.int64, scale=2.0):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    logits = torch.randn(rows, vocab, generator=g, device="cuda") * scale
+    teacher, indices = torch.topk(logits + torch.randn(rows, vocab, generator=g, device="cuda"), top, -1)
+    return logits.to(dtype), teacher.to(dtype), indices.to(index_dtype)
+
+
+def reference(logits, teacher, indices, temperature, reduction):
+    x = logits.detach().double().requires_grad_()
+    losses, counted = plain.distill(x, teacher.double(), indices, temperature)
+    if reduction == "none":
+        return losses, x
+    total = losses.sum()
+    return (total / max(1, sum(counted)) if reduction == "mean" else total), x
+
+
+SHAPES = [(5, 1000, 8), (1, 7, 7), (3, 1, 1), (4, 4099, 33), (2, 50001, 16), (9, 513, 300), (2, 32000, 64),
+          (150, 40, 3), (1, 130000, 5)]
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("temperature,reduction", [(1.0, "mean"), (2.5, "sum"), (0.7, "none")])
+@pytest.mark.parametrize("rows,vocab,top", SHAPES)
+def test_loss_and_gradient(rows, vocab, top, temperature, reduction, dtype):
+    logits, teacher, indices = inputs(rows, vocab, top, dtype, rows + vocab)
+    if rows > 2:
+        indices[1] = -1                    # a row without a teacher
+        teacher[2, top // 2:] = -math.inf  # one that gives fewer logits
+        if top == 1:
+            indices[2] = 0
+    want, x64 = reference(logits, teacher, indices, temperature, reduction)
+    x = logits.detach().requires_grad_()
+    loss = distillation_loss(x, teacher, indices, temperature=temperature, reduction=reduction)
+    assert loss.dtype == torch.float32 and loss.shape == want.shape
+    g = torch.Generator(device="cuda").manual_seed(3)
+    up = torch.randn(want.shape, generator=g, device="cuda")
+    plain_loss = distillation_loss(logits, teacher, indices, temperature=temperature, reduction=reduction)
+    assert torch.equal(plain_loss, loss.detach()) and not plain_loss.requires_grad
+    # a loss near zero is a difference of logarithms of the size of log V
+    assert float((loss.detach().double() - want.detach()).abs().max()) <= \
+        1e-5 * (float(want.detach().abs().max()) + temperature ** 2 * (rows if reduction == "sum" else 1))
+    if vocab == 1:
+        got = torch.autograd.grad(loss, x, up)[0]
+        assert not got.any()
+        return
+    got = torch.autograd.grad(loss, x, up)[0]
+    ref = torch.autograd.grad(want, x64, up.double())[0]
+    assert got.dtype == dtype and rel(got, ref) <= TOL[dtype]
+    if rows > 2:
+        assert not got[1].any()
+
+
+def test_gradient_against_differences():
+    logits, teacher, indices = inputs(3, 40, 6, torch.float32, 5)
+    x = logits.requires_grad_()
+    grad = torch.autograd.grad(distillation_loss(x, teacher, indices, temperature=1.7), x)[0].double()
+    g = torch.Generator(device="cuda").manual_seed(4)
+    direction = torch.randn(3, 40, generator=g, device="cuda").double()
+
+    def value(h):
+        losses, counted = plain.distill(logits.detach().double() + h * direction, teacher.double(), indices, 1.7)
+        return float(losses.sum()) / sum(counted)
+    want = (value(1e-6) - value(-1e-6)) / 2e-6
+    assert abs(float((grad * direction).sum()) - want) <= 1e-5 * float(grad.norm() * direction.norm())
+
+
+def test_upstream_factor_and_second_backward():
+    logits, teacher, indices = inputs(6, 300, 9, torch.float32, 6)
+    x = logits.requires_grad_()
+    loss = distillation_loss(x, teacher, indices)
+    once = torch.autograd.grad(loss, x, retain_graph=True)[0]
+    again = torch.autograd.grad(loss * 3.0, x, retain_graph=True)[0]
+    third = torch.autograd.grad(loss * -0.5, x)[0]
+    assert rel(again, 3.0 * once) <= 1e-6 and rel(third, -0.5 * once) <= 1e-6
+    assert once.data_ptr() != again.data_ptr()
+    loss = distillation_loss(x, teacher, indices)
+    assert rel(torch.autograd.grad(loss * 3.0, x)[0], 3.0 * once) <= 1e-6
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+def test_entries_named_twice_and_narrow_indices(dtype):
+    logits, teacher, indices = inputs(4, 100, 6, dtype, 7, index_dtype=torch.int32)
+    indices[0] = 5
+    indices[1, 3] = indices[1, 0]
+    indices[2, 1] = -7
+    want, x64 = reference(logits, teacher, indices, 1.0, "mean")
+    x = logits.requires_grad_()
+    loss = distillation_loss(x, teacher, indices)
+    assert abs(float(loss.detach()) - float(want.detach())) <= 1e-5 * (1 + abs(float(want.detach())))
+    assert rel(torch.autograd.grad(loss, x)[0], torch.autograd.grad(want, x64)[0]) <= TOL[dtype]
+
+
+def test_teacher_of_another_type():
+    logits, teacher, indices = inputs(4, 2000, 6, torch.bfloat16, 8)
+    teacher = teacher.float() + 0.01
+    want, x64 = reference(logits, teacher, indices, 1.0, "sum")
+    x = logits.requires_grad_()
+    loss = distillation_loss(x, teacher, indices, reduction="sum")
+    assert abs(float(loss.detach()) - float(want.detach())) <= 1e-5 * (4 + abs(float(want.detach())))
+    assert rel(torch.autograd.grad(loss, x)[0], torch.autograd.grad(want, x64)[0]) <= TOL[torch.bfloat16]
+
+
+@pytest.mark.parametrize("low", (-math.inf, torch.finfo(torch.bfloat16).min))
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+def test_masked_student_entries(dtype, low):
+    """Vocabulary entries masked with -inf or the lowest value have no
+    probability and no gradient; long stretches of them are skipped over."""
+    logits, teacher, indices = inputs(4, 3000, 6, dtype, 9)
+    mask = torch.ones(4, 3000, dtype=torch.bool, device="cuda")
+    mask.scatter_(1, indices, False)
+    mask[:, 2900:] = False
+    mask[3] = False
+    logits = logits.masked_fill(mask, low)
+    want, x64 = reference(logits, teacher, indices, 1.0, "mean")
+    x = logits.requires_grad_()
+    loss = distillation_loss(x, teacher, indices)
+    got = torch.autograd.grad(loss, x)[0]
+    assert abs(float(loss.detach()) - float(want.detach())) <= 1e-5 * (1 + abs(float(want.detach())))
+    ref = torch.autograd.grad(want, x64)[0]
+    assert torch.isfinite(got).all() and not got[mask].any()
+    assert rel(got, ref) <= TOL[dtype]
+
+
+def test_impossible_entries_and_not_a_number():
+    logits, teacher, indices = inputs(8, 500, 4, torch.float32, 10)
+    logits[0, indices[0, 0]] = -math.inf   # the teacher asks for what the student rules out
+    indices[1, 2] = 500                    # past the vocabulary
+    logits[2, 17] = math.nan
+    logits[3] = -math.inf
+    logits[4, 3] = math.inf
+    teacher[5, 1] = math.nan
+    logits[6] = math.nan
+    indices[6] = -1                        # no teacher: whatever the logits are
+    x = logits.requires_grad_()
+    loss = distillation_loss(x, teacher, indices, reduction="none")
+    grad = torch.autograd.grad(loss, x, torch.ones_like(loss))[0]
+    assert loss[0] == math.inf and torch.isfinite(grad[0]).all()
+    for r in (1, 2, 3, 4, 5):
+        assert torch.isnan(loss[r]), r
+    for r in (1, 2, 3, 4):
+        assert torch.isnan(grad[r]).all(), r
+    assert torch.isnan(grad[5, indices[5]]).all()
+    assert loss[6] == 0 and not grad[6].any()
+    want, x64 = reference(logits.detach()[7:], teacher[7:], indices[7:], 1.0, "sum")
+    assert abs(float(loss[7].detach()) - float(want.detach())) <= 1e-5 * (1 + abs(float(want.detach())))
+    assert rel(grad[7:], torch.autograd.grad(want, x64)[0]) <= 1e-5
+
+
+def test_no_row_has_a_teacher():
+    logits, teacher, indices = inputs(3, 100, 4, torch.float32, 11)
+    indices.fill_(-1)
+    x = logits.requires_grad_()
+    loss = distillation_loss(x, teacher, indices)
+    assert float(loss.detach()) == 0.0 and not torch.autograd.grad(loss, x)[0].any()
+    empty = torch.zeros(0, 100, device="cuda", requires_grad=True)
+    loss = distillation_loss(empty, teacher[:0], indices[:0])
+    assert float(loss.detach()) == 0.0 and torch.autograd.grad(loss, empty)[0].shape == (0, 100)
+
+
+def test_rows_of_a_padded_vocabulary_and_leading_dimensions():
+    g = torch.Generator(device="cuda").manual_seed(12)
+    wide = torch.randn(2, 5, 1032, generator=g, device="cuda", dtype=torch.bfloat16)
+    for lo, hi in ((0, 1000), (3, 1003), (8, 1032)):
+        logits = wide[..., lo:hi]
+        teacher, indices = torch.topk(logits.float(), 7, -1)
+        want, x64 = reference(logits.reshape(10, -1), teacher.reshape(10, -1), indices.reshape(10, -1), 1.0, "mean")
+        x = logits.detach().requires_grad_()
+        loss = distillation_loss(x, teacher, indices)
+        assert abs(float(loss.detach()) - float(want.detach())) <= 1e-5 * (1 + abs(float(want.detach())))
+        got = torch.autograd.grad(loss, x)[0]
+        assert rel(got.reshape(10, -1), torch.autograd.grad(want, x64)[0]) <= TOL[torch.bfloat16]
+
+
+def test_runs_are_identical_and_match_the_torch_form():
+    logits, teacher, indices = inputs(300, 5000, 20, torch.float32, 13)
+    x = logits.requires_grad_()
+    first = None
+    for _ in range(3):
+        loss = distillation_loss(x, teacher, indices, temperature=2.0)
+        got = (loss.detach(), torch.autograd.grad(loss, x)[0])
+        first = first or got
+        assert torch.equal(got[0], first[0]) and torch.equal(got[1], first[1])
+    loss = distillation_loss_torch(x, teacher, indices, temperature=2.0)
+    assert rel(first[0], loss) <= 1e-5 and rel(first[1], torch.autograd.grad(loss, x)[0]) <= 1e-5
+
+
+def test_refusals_on_the_gpu():
+    logits, teacher, indices = inputs(2, 3000, 4, torch.float32, 14)
+    with pytest.raises(NotImplementedError, match="at most 1024"):
+        distillation_loss(logits, logits[:, :2000], torch.arange(2000, device="cuda").expand(2, 2000))
+    with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+        distillation_loss(logits.double(), teacher, indices)
+    with pytest.raises(ValueError, match="same device"):
+        distillation_loss(logits, teacher, indices.cpu())
