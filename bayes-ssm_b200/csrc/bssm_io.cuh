@@ -58,7 +58,9 @@ template <typename T, int VEC> __device__ __forceinline__ void store_packed(T *p
     *reinterpret_cast<Packed<T, VEC> *>(p) = o;
 }
 
-__device__ __forceinline__ float sigmoid_f(float x) { return 1.f / (1.f + __expf(-x)); }
+// expf rather than __expf: the latter rounds x log2 e to float32 first, which
+// costs |x| 2^-24 of the result.
+__device__ __forceinline__ float sigmoid_f(float x) { return __fdividef(1.f, 1.f + expf(-x)); }
 
 // The sequences in the token rows: `count` runs of `length` tokens each, or,
 // with offsets (count + 1 int64 values from 0 to tokens, never decreasing),
