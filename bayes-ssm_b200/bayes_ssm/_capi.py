@@ -69,11 +69,12 @@ _SIGNATURES = {
                                   + [_l, _vp], _i),
     "bssm_causal_conv_step": ([_vp, _i, _l, _l, _i, _i, _vp, _i, _vp, _i, _i, _vp, _vp, _vp], _i),
     "bssm_selective_saved_floats": ([_l, _l, _i, _i], _l),
-    "bssm_selective_scan": ([_vp, _l] * 5 + [_i, _vp, _vp, _vp, _i, _l, _i, _i, _i, _vp, _l, _vp, _vp, _vp, _vp, _l,
-                                             _vp], _i),
-    "bssm_selective_backward_floats": ([_l, _l, _i, _i, _i], _l),
-    "bssm_selective_scan_backward": ([_vp, _l] * 5 + [_i, _vp, _vp, _vp, _i, _l, _i, _i, _i, _vp, _l] + [_vp] * 13
-                                     + [_l, _vp], _i),
+    "bssm_selective_scan_floats": ([_l, _l, _l, _i, _i, _i], _l),
+    "bssm_selective_scan": ([_vp, _l] * 5 + [_i, _vp, _vp, _vp, _i, _l, _i, _i, _i, _vp, _l, _l, _vp, _vp, _vp, _vp,
+                                             _l, _vp, _l, _vp], _i),
+    "bssm_selective_backward_floats": ([_l, _l, _l, _i, _i, _i], _l),
+    "bssm_selective_scan_backward": ([_vp, _l] * 5 + [_i, _vp, _vp, _vp, _i, _l, _i, _i, _i, _vp, _l, _l]
+                                     + [_vp] * 13 + [_l, _vp], _i),
     "bssm_selective_step": ([_vp, _l] * 5 + [_i, _vp, _vp, _vp, _i, _l, _i, _i, _i, _vp, _vp, _vp], _i),
     "bssm_distillation": ([_vp, _i, _l, _i, _l, _vp, _i, _vp, _i, _i, ctypes.c_float, _i, _vp, _vp, _vp, _vp, _vp,
                            _vp], _i),

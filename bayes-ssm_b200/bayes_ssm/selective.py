@@ -92,19 +92,19 @@ def _check_devices(first: Tensor, **others) -> None:
             raise ValueError(f"{name} must be on the same device as the rows")
 
 
-def _layout(lead: torch.Size, sequences: Optional[PackedSequences], device) -> tuple[int, int, Optional[int]]:
-    """Number of sequences, of token rows, and the offsets' address."""
+def _layout(lead: torch.Size, sequences: Optional[PackedSequences], device) -> tuple[int, int, int, Optional[int]]:
+    """Number of sequences, of token rows, the longest sequence, and the offsets' address."""
     if sequences is None:
         if len(lead) != 2:
             raise ValueError("rows must be [B, T, ...], or [tokens, ...] with sequences")
-        return lead[0], lead[0] * lead[1], None
+        return lead[0], lead[0] * lead[1], lead[1], None
     if not isinstance(sequences, PackedSequences):
         raise TypeError("sequences must be PackedSequences")
     if len(lead) != 1 or lead[0] != sequences.tokens:
         raise ValueError(f"rows must be [{sequences.tokens}, ...] for these sequences")
     if sequences.offsets.device != device:
         raise ValueError("sequences must be on the same device as the rows")
-    return sequences.count, sequences.tokens, sequences.offsets.data_ptr()
+    return sequences.count, sequences.tokens, sequences.longest, sequences.offsets.data_ptr()
 
 
 def _gradients_wanted(*tensors) -> bool:
@@ -236,7 +236,7 @@ def causal_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, *, act
     floating dtype than ``x``.
     """
     weight = _conv_arguments(x, weight, bias, activation)
-    count, tokens, offsets = _layout(x.shape[:-1], sequences, x.device)
+    count, tokens, _, offsets = _layout(x.shape[:-1], sequences, x.device)
     if initial_state is not None:
         if initial_state.shape != (count, weight.shape[1] - 1, x.shape[-1]):
             raise ValueError(f"initial_state must be [{count}, {weight.shape[1] - 1}, {x.shape[-1]}]")
@@ -377,8 +377,8 @@ def _scan_rows(values, steps, keys, queries, gate):
     return rows, [z for x, stride in rows for z in (_capi.ptr(x), stride)]
 
 
-def _scan_forward(values, steps, rates, keys, queries, skip, gate, step_bias, state, softplus, count, tokens, offsets,
-                  save):
+def _scan_forward(values, steps, rates, keys, queries, skip, gate, step_bias, state, softplus, count, tokens, longest,
+                  offsets, save):
     dev = values.device
     channels, n = rates.shape
     groups = keys.shape[-2]
@@ -393,11 +393,13 @@ def _scan_forward(values, steps, rates, keys, queries, skip, gate, step_bias, st
     if save:
         saved = torch.empty(lib.bssm_selective_saved_floats(tokens, count, channels, n), device=dev,
                             dtype=torch.float32)
+    room = lib.bssm_selective_scan_floats(tokens, count, longest, channels, n, groups)
+    ws = torch.empty(room, device=dev, dtype=torch.float32) if room else None
     with torch.cuda.device(dev):
         rc = lib.bssm_selective_scan(
             *flat, _DTYPES[values.dtype], rates.data_ptr(), _capi.ptr(skip), _capi.ptr(step_bias), int(softplus),
-            tokens, channels, n, groups, offsets, count, _capi.ptr(state), out.data_ptr(), final.data_ptr(),
-            _capi.ptr(saved), 0 if saved is None else saved.numel(), _stream(dev))
+            tokens, channels, n, groups, offsets, count, longest, _capi.ptr(state), out.data_ptr(), final.data_ptr(),
+            _capi.ptr(saved), 0 if saved is None else saved.numel(), _capi.ptr(ws), room, _stream(dev))
     _capi.check(rc, "bssm_selective_scan")
     del kept
     return out, final, saved
@@ -406,12 +408,12 @@ def _scan_forward(values, steps, rates, keys, queries, skip, gate, step_bias, st
 class _SelectiveScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, values, steps, rates, keys, queries, skip, gate, step_bias, state, softplus, count, tokens,
-                sequences):
+                longest, sequences):
         offsets = None if sequences is None else sequences.offsets.data_ptr()
         out, final, saved = _scan_forward(values, steps, rates, keys, queries, skip, gate, step_bias, state, softplus,
-                                          count, tokens, offsets, True)
+                                          count, tokens, longest, offsets, True)
         ctx.save_for_backward(values, steps, rates, keys, queries, skip, gate, step_bias, saved)
-        ctx.layout = (softplus, count, tokens, sequences, state is not None)
+        ctx.layout = (softplus, count, tokens, longest, sequences, state is not None)
         ctx.set_materialize_grads(False)
         return out, final
 
@@ -419,7 +421,7 @@ class _SelectiveScan(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gout, gfinal):
         values, steps, rates, keys, queries, skip, gate, step_bias, saved = ctx.saved_tensors
-        softplus, count, tokens, sequences, has_state = ctx.layout
+        softplus, count, tokens, longest, sequences, has_state = ctx.layout
         dev, dtype = values.device, values.dtype
         channels, n = rates.shape
         groups = keys.shape[-2]
@@ -439,18 +441,18 @@ class _SelectiveScan(torch.autograd.Function):
         gskip = None if skip is None else torch.empty(channels, device=dev, dtype=torch.float32)
         gbias = None if step_bias is None else torch.empty(channels, device=dev, dtype=torch.float32)
         g0 = torch.empty(count, channels, n, device=dev, dtype=torch.float32) if has_state else None
-        ws = torch.empty(lib.bssm_selective_backward_floats(tokens, count, channels, n, groups), device=dev,
+        ws = torch.empty(lib.bssm_selective_backward_floats(tokens, count, longest, channels, n, groups), device=dev,
                          dtype=torch.float32)
         with torch.cuda.device(dev):
             rc = lib.bssm_selective_scan_backward(
                 *flat, _DTYPES[dtype], a.data_ptr(), _capi.ptr(sk), _capi.ptr(sb), int(softplus), tokens, channels, n,
-                groups, None if sequences is None else sequences.offsets.data_ptr(), count, saved.data_ptr(),
-                _capi.ptr(gout), _capi.ptr(gfinal), gv.data_ptr(), gs.data_ptr(), ga.data_ptr(), gk.data_ptr(),
+                groups, None if sequences is None else sequences.offsets.data_ptr(), count, longest,
+                saved.data_ptr(), _capi.ptr(gout), _capi.ptr(gfinal), gv.data_ptr(), gs.data_ptr(), ga.data_ptr(), gk.data_ptr(),
                 gq.data_ptr(), _capi.ptr(gskip), _capi.ptr(gz), _capi.ptr(gbias), _capi.ptr(g0), ws.data_ptr(),
                 ws.numel(), _stream(dev))
         _capi.check(rc, "bssm_selective_scan_backward")
         del kept
-        return gv, gs, ga, gk, gq, gskip, gz, gbias, g0, None, None, None, None
+        return gv, gs, ga, gk, gq, gskip, gz, gbias, g0, None, None, None, None, None
 
 
 def selective_scan(values: Tensor, steps: Tensor, rates: Tensor, keys: Tensor, queries: Tensor, *,
@@ -468,7 +470,7 @@ def selective_scan(values: Tensor, steps: Tensor, rates: Tensor, keys: Tensor, q
     A token whose step is zero leaves the state as it is.
     """
     rates, keys, queries, skip, step_bias = _scan_arguments(values, steps, rates, keys, queries, skip, gate, step_bias)
-    count, tokens, offsets = _layout(values.shape[:-1], sequences, values.device)
+    count, tokens, longest, offsets = _layout(values.shape[:-1], sequences, values.device)
     if initial_state is not None:
         if initial_state.shape != (count, *rates.shape):
             raise ValueError(f"initial_state must be [{count}, {rates.shape[0]}, {rates.shape[1]}]")
@@ -480,8 +482,8 @@ def selective_scan(values: Tensor, steps: Tensor, rates: Tensor, keys: Tensor, q
         initial_state = initial_state.float()
     args = (values, steps, rates, keys, queries, skip, gate, step_bias, initial_state)
     if _gradients_wanted(*args):
-        return _SelectiveScan.apply(*args, bool(softplus), count, tokens, sequences)
-    return _scan_forward(*args, bool(softplus), count, tokens, offsets, False)[:2]
+        return _SelectiveScan.apply(*args, bool(softplus), count, tokens, longest, sequences)
+    return _scan_forward(*args, bool(softplus), count, tokens, longest, offsets, False)[:2]
 
 
 def selective_step(values: Tensor, steps: Tensor, rates: Tensor, keys: Tensor, queries: Tensor, state: Tensor, *,

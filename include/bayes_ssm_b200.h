@@ -463,6 +463,9 @@ int bssm_causal_conv_step(const void *x, int dtype, long row_stride, long sequen
  * shared by channels / groups adjacent channels; rates [channels][states],
  * skip and step_bias [channels] (may be null) float32; state0 (null: zeros)
  * and state1 [sequences][channels][states] float32, state1 16-byte aligned.
+ * longest is the longest sequence's tokens (it sets how sequences are split
+ * over CTAs; the same value goes to the workspace query and the call).
+ * workspace (16-byte aligned): bssm_selective_scan_floats() floats, maybe 0.
  * saved (16-byte aligned, bssm_selective_saved_floats() floats; null where no
  * backward follows) receives the states the backward starts its replays from;
  * its layout is internal.
@@ -473,19 +476,22 @@ int bssm_causal_conv_step(const void *x, int dtype, long row_stride, long sequen
  * on in place.
  */
 long bssm_selective_saved_floats(long tokens, long sequences, int channels, int states);
+long bssm_selective_scan_floats(long tokens, long sequences, long longest, int channels, int states, int groups);
 int bssm_selective_scan(const void *values, long value_stride, const void *steps, long step_stride, const void *keys,
                         long key_stride, const void *queries, long query_stride, const void *gate, long gate_stride,
                         int dtype, const float *rates, const float *skip, const float *step_bias, int softplus,
                         long tokens, int channels, int states, int groups, const long *offsets, long sequences,
-                        const float *state0, void *out, float *state1, float *saved, long saved_floats, void *stream);
-long bssm_selective_backward_floats(long tokens, long sequences, int channels, int states, int groups);
+                        long longest, const float *state0, void *out, float *state1, float *saved, long saved_floats,
+                        float *workspace, long workspace_floats, void *stream);
+long bssm_selective_backward_floats(long tokens, long sequences, long longest, int channels, int states, int groups);
 int bssm_selective_scan_backward(
     const void *values, long value_stride, const void *steps, long step_stride, const void *keys, long key_stride,
     const void *queries, long query_stride, const void *gate, long gate_stride, int dtype, const float *rates,
     const float *skip, const float *step_bias, int softplus, long tokens, int channels, int states, int groups,
-    const long *offsets, long sequences, const float *saved, const void *grad_out, const float *grad_state1,
-    void *grad_values, void *grad_steps, float *grad_rates, void *grad_keys, void *grad_queries, float *grad_skip,
-    void *grad_gate, float *grad_step_bias, float *grad_state0, float *workspace, long workspace_floats, void *stream);
+    const long *offsets, long sequences, long longest, const float *saved, const void *grad_out,
+    const float *grad_state1, void *grad_values, void *grad_steps, float *grad_rates, void *grad_keys,
+    void *grad_queries, float *grad_skip, void *grad_gate, float *grad_step_bias, float *grad_state0, float *workspace,
+    long workspace_floats, void *stream);
 int bssm_selective_step(const void *values, long value_stride, const void *steps, long step_stride, const void *keys,
                         long key_stride, const void *queries, long query_stride, const void *gate, long gate_stride,
                         int dtype, const float *rates, const float *skip, const float *step_bias, int softplus,
