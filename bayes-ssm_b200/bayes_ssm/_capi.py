@@ -76,6 +76,7 @@ _SIGNATURES = {
     "bssm_selective_scan_backward": ([_vp, _l] * 5 + [_i, _vp, _vp, _vp, _i, _l, _i, _i, _i, _vp, _l, _l]
                                      + [_vp] * 13 + [_l, _vp], _i),
     "bssm_selective_step": ([_vp, _l] * 5 + [_i, _vp, _vp, _vp, _i, _l, _i, _i, _i, _vp, _vp, _vp], _i),
+    "bssm_distillation_counters": ([], _i),
     "bssm_distillation": ([_vp, _i, _l, _i, _l, _vp, _i, _vp, _i, _i, ctypes.c_float, _i, _vp, _vp, _vp, _vp, _vp,
                            _vp], _i),
     "bssm_distillation_backward": ([_vp, _i, _l, _i, _l, _vp, _i, _vp, _i, _i, ctypes.c_float, _i, _vp, _vp, _vp, _i,
@@ -123,6 +124,21 @@ def check(rc: int, what: str) -> None:
 def ptr(t) -> Optional[int]:
     """Device pointer of a tensor (None passes NULL)."""
     return None if t is None else t.data_ptr()
+
+
+def launch(device, name: str, *args) -> None:
+    """Call the entry point ``name`` with ``args`` and ``device``'s current
+    stream as its last argument, and raise on a non-zero status."""
+    import torch
+    fn = getattr(_LIB or load(), name)
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, name)
 
 
 def forward_chunked(key_dim, value_dim, io_dtype, fixed, keys, values, queries, decay, process,

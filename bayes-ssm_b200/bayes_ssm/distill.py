@@ -19,7 +19,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _capi
-from .selective import _DTYPES, _gradients_wanted, _rows, _stream
+from .selective import _DTYPES, _empty_like, _gradients_wanted, _rows
 
 MAX_TOP = 1024
 
@@ -49,60 +49,58 @@ def distillation_loss_torch(logits: Tensor, teacher_logits: Tensor, teacher_indi
     return total / counted.sum().clamp(min=1) if reduction == "mean" else total
 
 
+def _forward(logits, teacher, indices, temperature, reduction, with_grad):
+    """Loss (of every row, or reduced), its gradient where it is wanted and
+    known up to a factor, and what the backward needs otherwise."""
+    dev = logits.device
+    vocab, top = logits.shape[-1], teacher.shape[-1]
+    rows = teacher.numel() // top
+    x, stride = _rows(logits, 1)
+    mean, reduced = reduction == "mean", reduction != "none"
+    # statistics (2 floats a row), row losses, partial counts
+    scratch = torch.empty(3 * rows + _capi.load().bssm_distillation_counters(), device=dev, dtype=torch.float32)
+    at = scratch.data_ptr()
+    loss = torch.empty(() if reduced else logits.shape[:-1], device=dev, dtype=torch.float32)
+    grad = _empty_like(logits) if with_grad and reduced else None
+    _capi.launch(dev, "bssm_distillation", x.data_ptr(), _DTYPES[x.dtype], rows, vocab, stride, teacher.data_ptr(),
+                 _DTYPES[teacher.dtype], indices.data_ptr(), indices.element_size(), top, temperature, mean,
+                 at + 8 * rows if reduced else loss.data_ptr(), at, loss.data_ptr() if reduced else None,
+                 at + 12 * rows, _capi.ptr(grad))
+    return loss, grad, scratch
+
+
 class _Distillation(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, teacher, indices, temperature, reduction, with_grad):
-        dev = logits.device
-        vocab, top = logits.shape[-1], teacher.shape[-1]
-        rows = teacher.numel() // top
-        x, stride = _rows(logits, 1)
-        teacher, indices = teacher.contiguous(), indices.contiguous()
-        mean, reduced = int(reduction == "mean"), reduction != "none"
-        stats = torch.empty(rows, 2, device=dev, dtype=torch.float32)
-        row_loss = torch.empty(logits.shape[:-1], device=dev, dtype=torch.float32)
-        loss = torch.empty((), device=dev, dtype=torch.float32) if reduced else None
-        count = torch.empty(1, device=dev, dtype=torch.int32)
-        # one number: its gradient is known here up to a factor
-        grad = torch.empty(logits.shape, device=dev, dtype=logits.dtype) if with_grad and reduced else None
-        with torch.cuda.device(dev):
-            rc = _capi.load().bssm_distillation(
-                x.data_ptr(), _DTYPES[x.dtype], rows, vocab, stride, teacher.data_ptr(), _DTYPES[teacher.dtype],
-                indices.data_ptr(), indices.element_size(), top, temperature, mean, row_loss.data_ptr(),
-                stats.data_ptr(), _capi.ptr(loss), count.data_ptr(), _capi.ptr(grad), _stream(dev))
-        _capi.check(rc, "bssm_distillation")
-        if with_grad:
-            ctx.save_for_backward(logits, teacher, indices, stats, count)
-            ctx.settings = (temperature, mean, reduced)
-            ctx.grad = grad
-        return loss if reduced else row_loss
+    def forward(ctx, logits, teacher, indices, temperature, reduction):
+        loss, ctx.grad, scratch = _forward(logits, teacher, indices, temperature, reduction, True)
+        ctx.save_for_backward(logits, teacher, indices, scratch)
+        ctx.settings = (temperature, reduction)
+        return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, upstream):
-        logits, teacher, indices, stats, count = ctx.saved_tensors
-        temperature, mean, reduced = ctx.settings
+        logits, teacher, indices, scratch = ctx.saved_tensors
+        temperature, reduction = ctx.settings
         dev = logits.device
         upstream = upstream.float().contiguous()
         # The gradient written by the forward is handed out once, times the
         # upstream one; a second walk through a retained graph makes its own.
         grad, ctx.grad = ctx.grad, None
-        with torch.cuda.device(dev):
-            lib = _capi.load()
-            if grad is not None:
-                rc = lib.bssm_distillation_scale(grad.data_ptr(), _DTYPES[grad.dtype], grad.numel(),
-                                                 upstream.data_ptr(), _stream(dev))
-                _capi.check(rc, "bssm_distillation_scale")
-            else:
-                x, stride = _rows(logits, 1)
-                top = teacher.shape[-1]
-                grad = torch.empty(logits.shape, device=dev, dtype=logits.dtype)
-                rc = lib.bssm_distillation_backward(
-                    x.data_ptr(), _DTYPES[x.dtype], teacher.numel() // top, logits.shape[-1], stride,
-                    teacher.data_ptr(), _DTYPES[teacher.dtype], indices.data_ptr(), indices.element_size(), top,
-                    temperature, mean, stats.data_ptr(), count.data_ptr(), upstream.data_ptr(), int(not reduced),
-                    grad.data_ptr(), _stream(dev))
-                _capi.check(rc, "bssm_distillation_backward")
-        return grad, None, None, None, None, None
+        if grad is not None:
+            _capi.launch(dev, "bssm_distillation_scale", grad.data_ptr(), _DTYPES[grad.dtype], grad.numel(),
+                         upstream.data_ptr())
+            return grad, None, None, None, None
+        x, stride = _rows(logits, 1)
+        top = teacher.shape[-1]
+        rows = teacher.numel() // top
+        grad = _empty_like(logits)
+        at = scratch.data_ptr()
+        _capi.launch(dev, "bssm_distillation_backward", x.data_ptr(), _DTYPES[x.dtype], rows, logits.shape[-1],
+                     stride, teacher.data_ptr(), _DTYPES[teacher.dtype], indices.data_ptr(), indices.element_size(),
+                     top, temperature, reduction == "mean", at, at + 12 * rows, upstream.data_ptr(),
+                     reduction == "none", grad.data_ptr())
+        return grad, None, None, None, None
 
 
 def distillation_loss(logits: Tensor, teacher_logits: Tensor, teacher_indices: Tensor, *, temperature: float = 1.0,
@@ -144,8 +142,10 @@ def distillation_loss(logits: Tensor, teacher_logits: Tensor, teacher_indices: T
     if teacher_logits.shape[-1] > MAX_TOP:
         raise NotImplementedError(f"distillation_loss on CUDA needs at most {MAX_TOP} teacher logits a row "
                                   f"(got {teacher_logits.shape[-1]}); use distillation_loss_torch")
-    return _Distillation.apply(logits, teacher_logits.detach(), teacher_indices, float(temperature), reduction,
-                               _gradients_wanted(logits))
+    teacher, indices = teacher_logits.detach().contiguous(), teacher_indices.contiguous()
+    if _gradients_wanted(logits):
+        return _Distillation.apply(logits, teacher, indices, float(temperature), reduction)
+    return _forward(logits, teacher, indices, float(temperature), reduction, False)[0]
 
 
 __all__ = ["distillation_loss", "distillation_loss_torch"]

@@ -66,11 +66,13 @@ class PackedSequences:
 def _rows(x: Tensor, trailing: int) -> tuple[Tensor, int]:
     """``x`` with its trailing dimensions contiguous and its rows evenly
     spaced (a copy where they are not), and the spacing in elements."""
-    inner, even = 1, True
+    inner = x.shape[-1] if trailing == 1 else x.shape[-1] * x.shape[-2]
+    if x.is_contiguous():
+        return x, inner
     sizes, strides = x.shape, x.stride()
-    for size, stride in zip(reversed(sizes[-trailing:]), reversed(strides[-trailing:])):
-        even &= size == 1 or stride == inner
-        inner *= size
+    even = sizes[-1] == 1 or strides[-1] == 1
+    if trailing == 2:
+        even &= sizes[-2] == 1 or strides[-2] == sizes[-1]
     row = expect = None
     for size, stride in zip(reversed(sizes[:-trailing]), reversed(strides[:-trailing])):
         if size == 1:
@@ -86,9 +88,14 @@ def _rows(x: Tensor, trailing: int) -> tuple[Tensor, int]:
     return x, row
 
 
+def _empty_like(x: Tensor) -> Tensor:
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, device=x.device, dtype=x.dtype)
+
+
 def _check_devices(first: Tensor, **others) -> None:
+    device = first.device
     for name, x in others.items():
-        if x is not None and x.device != first.device:
+        if x is not None and x.device != device:
             raise ValueError(f"{name} must be on the same device as the rows")
 
 
@@ -108,11 +115,11 @@ def _layout(lead: torch.Size, sequences: Optional[PackedSequences], device) -> t
 
 
 def _gradients_wanted(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in tensors)
-
-
-def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    if torch.is_grad_enabled():
+        for x in tensors:
+            if x is not None and x.requires_grad:
+                return True
+    return False
 
 
 # ---------------------------------------------------------------------------
@@ -129,11 +136,11 @@ def _conv_arguments(x, weight, bias, activation):
         raise ValueError(f"bias must be [{channels}]")
     if activation not in (None, "silu"):
         raise ValueError("activation must be None or 'silu'")
-    if not all(t is None or t.is_floating_point() for t in (x, weight, bias)):
+    if not (x.is_floating_point() and weight.is_floating_point() and (bias is None or bias.is_floating_point())):
         raise TypeError("x, weight and bias must have floating-point dtype")
     _check_devices(x, weight=weight, bias=bias)
     if x.is_cuda:
-        if any(t is not None and t.dtype not in _DTYPES for t in (x, weight, bias)):
+        if x.dtype not in _DTYPES or weight.dtype not in _DTYPES or (bias is not None and bias.dtype not in _DTYPES):
             raise TypeError("causal_conv on CUDA takes float32, bfloat16 or float16 tensors")
         if not 2 <= weight.shape[1] <= 4:
             raise NotImplementedError(f"causal_conv on CUDA needs 2, 3 or 4 taps (got {weight.shape[1]}); "
@@ -172,14 +179,12 @@ def _conv_forward(x, weight, bias, silu, state, count, tokens, offsets):
     weight = weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     state = None if state is None else state.contiguous()
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    y = _empty_like(x)
     final = torch.empty(count, taps - 1, channels, device=x.device, dtype=x.dtype)
-    with torch.cuda.device(x.device):
-        rc = _capi.load().bssm_causal_conv(
-            x.data_ptr(), _DTYPES[x.dtype], stride, tokens, channels, taps, weight.data_ptr(), _DTYPES[weight.dtype],
-            _capi.ptr(bias), 0 if bias is None else _DTYPES[bias.dtype], silu, offsets, count, _capi.ptr(state),
-            y.data_ptr(), final.data_ptr(), _stream(x.device))
-    _capi.check(rc, "bssm_causal_conv")
+    _capi.launch(x.device, "bssm_causal_conv", x.data_ptr(), _DTYPES[x.dtype], stride, tokens, channels, taps,
+                 weight.data_ptr(), _DTYPES[weight.dtype], _capi.ptr(bias),
+                 0 if bias is None else _DTYPES[bias.dtype], silu, offsets, count, _capi.ptr(state), y.data_ptr(),
+                 final.data_ptr())
     return y, final
 
 
@@ -205,20 +210,16 @@ class _CausalConv(torch.autograd.Function):
         wt = weight.contiguous()
         b = None if bias is None else bias.contiguous()
         past = None if state is None else state.contiguous()
-        gx = torch.empty(x.shape, device=dev, dtype=x.dtype)
-        gw = torch.empty(channels, taps, device=dev, dtype=weight.dtype)
-        gb = None if bias is None else torch.empty(channels, device=dev, dtype=bias.dtype)
-        gs = None if state is None else torch.empty(past.shape, device=dev, dtype=x.dtype)
-        lib = _capi.load()
-        ws = torch.empty(lib.bssm_causal_conv_partial_floats(tokens, channels, taps), device=dev, dtype=torch.float32)
-        with torch.cuda.device(dev):
-            rc = lib.bssm_causal_conv_backward(
-                rows.data_ptr(), _DTYPES[x.dtype], stride, tokens, channels, taps, wt.data_ptr(), _DTYPES[wt.dtype],
-                _capi.ptr(b), 0 if b is None else _DTYPES[b.dtype], silu,
-                None if sequences is None else sequences.offsets.data_ptr(), count, _capi.ptr(past), gy.data_ptr(),
-                _capi.ptr(gfinal), gx.data_ptr(), gw.data_ptr(), _capi.ptr(gb), _capi.ptr(gs), ws.data_ptr(),
-                ws.numel(), _stream(dev))
-        _capi.check(rc, "bssm_causal_conv_backward")
+        gx, gw = _empty_like(rows), _empty_like(wt)
+        gb = None if b is None else torch.empty_like(b)
+        gs = None if past is None else torch.empty_like(past)
+        room = _capi.load().bssm_causal_conv_partial_floats(tokens, channels, taps)
+        ws = torch.empty(room, device=dev, dtype=torch.float32)
+        _capi.launch(dev, "bssm_causal_conv_backward", rows.data_ptr(), _DTYPES[x.dtype], stride, tokens, channels,
+                     taps, wt.data_ptr(), _DTYPES[wt.dtype], _capi.ptr(b), 0 if b is None else _DTYPES[b.dtype], silu,
+                     None if sequences is None else sequences.offsets.data_ptr(), count, _capi.ptr(past),
+                     gy.data_ptr(), _capi.ptr(gfinal), gx.data_ptr(), gw.data_ptr(), _capi.ptr(gb), _capi.ptr(gs),
+                     ws.data_ptr(), room)
         return gx, gw, gb, gs, None, None, None, None
 
 
@@ -275,13 +276,11 @@ def causal_conv_step(x: Tensor, state: Tensor, weight: Tensor, bias: Optional[Te
     x, stride = _rows(x, 1)
     weight = weight.contiguous()
     bias = None if bias is None else bias.contiguous()
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    with torch.cuda.device(x.device):
-        rc = _capi.load().bssm_causal_conv_step(
-            x.data_ptr(), _DTYPES[x.dtype], stride, x.shape[0], x.shape[1], weight.shape[1], weight.data_ptr(),
-            _DTYPES[weight.dtype], _capi.ptr(bias), 0 if bias is None else _DTYPES[bias.dtype],
-            int(activation == "silu"), state.data_ptr(), y.data_ptr(), _stream(x.device))
-    _capi.check(rc, "bssm_causal_conv_step")
+    y = _empty_like(x)
+    _capi.launch(x.device, "bssm_causal_conv_step", x.data_ptr(), _DTYPES[x.dtype], stride, x.shape[0], x.shape[1],
+                 weight.shape[1], weight.data_ptr(), _DTYPES[weight.dtype], _capi.ptr(bias),
+                 0 if bias is None else _DTYPES[bias.dtype], int(activation == "silu"), state.data_ptr(),
+                 y.data_ptr())
     return y
 
 
@@ -290,33 +289,35 @@ def causal_conv_step(x: Tensor, state: Tensor, weight: Tensor, bias: Optional[Te
 # ---------------------------------------------------------------------------
 
 def _scan_arguments(values, steps, rates, keys, queries, skip, gate, step_bias):
-    """Shapes, dtypes and devices; returns keys and queries as [..., G, N] and the per-channel tensors in float32."""
-    lead, channels = values.shape[:-1], values.shape[-1]
-    if not all(t is None or t.is_floating_point() for t in (values, steps, rates, keys, queries, skip, gate,
-                                                            step_bias)):
-        raise TypeError("selective_scan takes floating-point tensors")
-    if steps.shape != values.shape or (gate is not None and gate.shape != values.shape):
+    """Checks shapes, dtypes and devices; returns the groups of keys and queries, and the per-channel tensors in
+    float32 (on CUDA)."""
+    shape, dtype, lead = values.shape, values.dtype, values.ndim - 1
+    channels = shape[-1]
+    for x in (values, steps, rates, keys, queries, skip, gate, step_bias):
+        if x is not None and not x.is_floating_point():
+            raise TypeError("selective_scan takes floating-point tensors")
+    if steps.shape != shape or (gate is not None and gate.shape != shape):
         raise ValueError("steps and gate must have the values' shape")
     if rates.ndim != 2 or rates.shape[0] != channels or rates.shape[1] < 1:
         raise ValueError(f"rates must be [{channels}, N]")
     n = rates.shape[1]
-    if keys.ndim == len(lead) + 1:
-        keys = keys.unsqueeze(-2)
-    if queries.ndim == len(lead) + 1:
-        queries = queries.unsqueeze(-2)
-    if keys.shape != queries.shape or keys.shape[:-2] != lead or keys.shape[-1] != n or keys.ndim != len(lead) + 2:
+    groups = keys.shape[-2] if keys.ndim == lead + 2 else 1
+    if keys.shape != queries.shape or keys.ndim not in (lead + 1, lead + 2) or keys.shape[:lead] != shape[:lead] \
+            or keys.shape[-1] != n:
         raise ValueError(f"keys and queries must be [..., {n}] or [..., G, {n}] with the values' leading dimensions")
-    if keys.shape[-2] < 1 or channels % keys.shape[-2]:
+    if groups < 1 or channels % groups:
         raise ValueError("the groups of keys and queries must divide the channels")
-    for name, x in (("skip", skip), ("step_bias", step_bias)):
-        if x is not None and x.shape != (channels,):
-            raise ValueError(f"{name} must be [{channels}]")
-    if any(t is not None and t.dtype != values.dtype for t in (steps, keys, queries, gate)):
+    if skip is not None and skip.shape != (channels,):
+        raise ValueError(f"skip must be [{channels}]")
+    if step_bias is not None and step_bias.shape != (channels,):
+        raise ValueError(f"step_bias must be [{channels}]")
+    if steps.dtype != dtype or keys.dtype != dtype or queries.dtype != dtype or (gate is not None
+                                                                                and gate.dtype != dtype):
         raise TypeError("values, steps, keys, queries and gate must have one dtype")
     _check_devices(values, steps=steps, rates=rates, keys=keys, queries=queries, skip=skip, gate=gate,
                    step_bias=step_bias)
     if values.is_cuda:
-        if values.dtype not in _DTYPES:
+        if dtype not in _DTYPES:
             raise TypeError("selective_scan on CUDA takes float32, bfloat16 or float16 rows")
         if n > MAX_STATES:
             raise NotImplementedError(f"selective_scan on CUDA needs at most {MAX_STATES} states (got {n}); "
@@ -324,7 +325,7 @@ def _scan_arguments(values, steps, rates, keys, queries, skip, gate, step_bias):
         rates = rates.float()
         skip = None if skip is None else skip.float()
         step_bias = None if step_bias is None else step_bias.float()
-    return rates, keys, queries, skip, step_bias
+    return groups, rates, skip, step_bias
 
 
 def selective_scan_torch(values: Tensor, steps: Tensor, rates: Tensor, keys: Tensor, queries: Tensor, *,
@@ -371,49 +372,49 @@ def selective_scan_torch(values: Tensor, steps: Tensor, rates: Tensor, keys: Ten
 
 
 def _scan_rows(values, steps, keys, queries, gate):
-    """The row arguments as (tensor, spacing), flat for the C call (tensors kept alive by the caller)."""
-    rows = [_rows(values, 1), _rows(steps, 1), _rows(keys, 2), _rows(queries, 2),
-            (None, 0) if gate is None else _rows(gate, 1)]
-    return rows, [z for x, stride in rows for z in (_capi.ptr(x), stride)]
+    """The row arguments (kept alive by the caller) and, for the C call, their addresses and spacings."""
+    trailing = keys.ndim - values.ndim + 1
+    x, xs = _rows(values, 1)
+    s, ss = _rows(steps, 1)
+    k, ks = _rows(keys, trailing)
+    q, qs = _rows(queries, trailing)
+    z, zs = (None, 0) if gate is None else _rows(gate, 1)
+    return (x, s, k, q, z), (x.data_ptr(), xs, s.data_ptr(), ss, k.data_ptr(), ks, q.data_ptr(), qs, _capi.ptr(z), zs)
 
 
-def _scan_forward(values, steps, rates, keys, queries, skip, gate, step_bias, state, softplus, count, tokens, longest,
-                  offsets, save):
+def _scan_forward(values, steps, rates, keys, queries, skip, gate, step_bias, state, groups, softplus, count, tokens,
+                  longest, offsets, save):
     dev = values.device
     channels, n = rates.shape
-    groups = keys.shape[-2]
     lib = _capi.load()
     kept, flat = _scan_rows(values, steps, keys, queries, gate)
     rates, state = rates.contiguous(), None if state is None else state.contiguous()
     skip = None if skip is None else skip.contiguous()
     step_bias = None if step_bias is None else step_bias.contiguous()
-    out = torch.empty(values.shape, device=dev, dtype=values.dtype)
+    out = _empty_like(values)
     final = torch.empty(count, channels, n, device=dev, dtype=torch.float32)
-    saved = None
-    if save:
-        saved = torch.empty(lib.bssm_selective_saved_floats(tokens, count, channels, n), device=dev,
-                            dtype=torch.float32)
     room = lib.bssm_selective_scan_floats(tokens, count, longest, channels, n, groups)
     ws = torch.empty(room, device=dev, dtype=torch.float32) if room else None
-    with torch.cuda.device(dev):
-        rc = lib.bssm_selective_scan(
-            *flat, _DTYPES[values.dtype], rates.data_ptr(), _capi.ptr(skip), _capi.ptr(step_bias), int(softplus),
-            tokens, channels, n, groups, offsets, count, longest, _capi.ptr(state), out.data_ptr(), final.data_ptr(),
-            _capi.ptr(saved), 0 if saved is None else saved.numel(), _capi.ptr(ws), room, _stream(dev))
-    _capi.check(rc, "bssm_selective_scan")
+    saved, saved_room = None, 0
+    if save:
+        saved_room = lib.bssm_selective_saved_floats(tokens, count, channels, n)
+        saved = torch.empty(saved_room, device=dev, dtype=torch.float32)
+    _capi.launch(dev, "bssm_selective_scan", *flat, _DTYPES[values.dtype], rates.data_ptr(), _capi.ptr(skip),
+                 _capi.ptr(step_bias), softplus, tokens, channels, n, groups, offsets, count, longest,
+                 _capi.ptr(state), out.data_ptr(), final.data_ptr(), _capi.ptr(saved), saved_room, _capi.ptr(ws), room)
     del kept
     return out, final, saved
 
 
 class _SelectiveScan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, values, steps, rates, keys, queries, skip, gate, step_bias, state, softplus, count, tokens,
-                longest, sequences):
+    def forward(ctx, values, steps, rates, keys, queries, skip, gate, step_bias, state, groups, softplus, count,
+                tokens, longest, sequences):
         offsets = None if sequences is None else sequences.offsets.data_ptr()
-        out, final, saved = _scan_forward(values, steps, rates, keys, queries, skip, gate, step_bias, state, softplus,
-                                          count, tokens, longest, offsets, True)
+        out, final, saved = _scan_forward(values, steps, rates, keys, queries, skip, gate, step_bias, state, groups,
+                                          softplus, count, tokens, longest, offsets, True)
         ctx.save_for_backward(values, steps, rates, keys, queries, skip, gate, step_bias, saved)
-        ctx.layout = (softplus, count, tokens, longest, sequences, state is not None)
+        ctx.layout = (groups, softplus, count, tokens, longest, sequences, state is not None)
         ctx.set_materialize_grads(False)
         return out, final
 
@@ -421,38 +422,31 @@ class _SelectiveScan(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gout, gfinal):
         values, steps, rates, keys, queries, skip, gate, step_bias, saved = ctx.saved_tensors
-        softplus, count, tokens, longest, sequences, has_state = ctx.layout
+        groups, softplus, count, tokens, longest, sequences, has_state = ctx.layout
         dev, dtype = values.device, values.dtype
         channels, n = rates.shape
-        groups = keys.shape[-2]
-        lib = _capi.load()
         kept, flat = _scan_rows(values, steps, keys, queries, gate)
         a = rates.contiguous()
         sk = None if skip is None else skip.contiguous()
         sb = None if step_bias is None else step_bias.contiguous()
         gout = None if gout is None else gout.to(dtype).contiguous()
         gfinal = None if gfinal is None else gfinal.float().contiguous()
-
-        def rows_like(x):
-            return None if x is None else torch.empty(x.shape, device=dev, dtype=dtype)
-
-        gv, gs, gk, gq, gz = (rows_like(x) for x in (values, steps, keys, queries, gate))
-        ga = torch.empty(channels, n, device=dev, dtype=torch.float32)
-        gskip = None if skip is None else torch.empty(channels, device=dev, dtype=torch.float32)
-        gbias = None if step_bias is None else torch.empty(channels, device=dev, dtype=torch.float32)
+        gv, gs, gk, gq = _empty_like(values), _empty_like(steps), _empty_like(keys), _empty_like(queries)
+        gz = None if gate is None else _empty_like(gate)
+        ga = torch.empty_like(a)
+        gskip = None if sk is None else torch.empty_like(sk)
+        gbias = None if sb is None else torch.empty_like(sb)
         g0 = torch.empty(count, channels, n, device=dev, dtype=torch.float32) if has_state else None
-        ws = torch.empty(lib.bssm_selective_backward_floats(tokens, count, longest, channels, n, groups), device=dev,
-                         dtype=torch.float32)
-        with torch.cuda.device(dev):
-            rc = lib.bssm_selective_scan_backward(
-                *flat, _DTYPES[dtype], a.data_ptr(), _capi.ptr(sk), _capi.ptr(sb), int(softplus), tokens, channels, n,
-                groups, None if sequences is None else sequences.offsets.data_ptr(), count, longest,
-                saved.data_ptr(), _capi.ptr(gout), _capi.ptr(gfinal), gv.data_ptr(), gs.data_ptr(), ga.data_ptr(), gk.data_ptr(),
-                gq.data_ptr(), _capi.ptr(gskip), _capi.ptr(gz), _capi.ptr(gbias), _capi.ptr(g0), ws.data_ptr(),
-                ws.numel(), _stream(dev))
-        _capi.check(rc, "bssm_selective_scan_backward")
+        room = _capi.load().bssm_selective_backward_floats(tokens, count, longest, channels, n, groups)
+        ws = torch.empty(room, device=dev, dtype=torch.float32)
+        _capi.launch(dev, "bssm_selective_scan_backward", *flat, _DTYPES[dtype], a.data_ptr(), _capi.ptr(sk),
+                     _capi.ptr(sb), softplus, tokens, channels, n, groups,
+                     None if sequences is None else sequences.offsets.data_ptr(), count, longest, saved.data_ptr(),
+                     _capi.ptr(gout), _capi.ptr(gfinal), gv.data_ptr(), gs.data_ptr(), ga.data_ptr(), gk.data_ptr(),
+                     gq.data_ptr(), _capi.ptr(gskip), _capi.ptr(gz), _capi.ptr(gbias), _capi.ptr(g0), ws.data_ptr(),
+                     room)
         del kept
-        return gv, gs, ga, gk, gq, gskip, gz, gbias, g0, None, None, None, None, None
+        return gv, gs, ga, gk, gq, gskip, gz, gbias, g0, None, None, None, None, None, None
 
 
 def selective_scan(values: Tensor, steps: Tensor, rates: Tensor, keys: Tensor, queries: Tensor, *,
@@ -469,7 +463,7 @@ def selective_scan(values: Tensor, steps: Tensor, rates: Tensor, keys: Tensor, q
     and ``final_state`` are float32 ``[B, C, N]``.  CUDA takes up to 64 states.
     A token whose step is zero leaves the state as it is.
     """
-    rates, keys, queries, skip, step_bias = _scan_arguments(values, steps, rates, keys, queries, skip, gate, step_bias)
+    groups, rates, skip, step_bias = _scan_arguments(values, steps, rates, keys, queries, skip, gate, step_bias)
     count, tokens, longest, offsets = _layout(values.shape[:-1], sequences, values.device)
     if initial_state is not None:
         if initial_state.shape != (count, *rates.shape):
@@ -482,8 +476,8 @@ def selective_scan(values: Tensor, steps: Tensor, rates: Tensor, keys: Tensor, q
         initial_state = initial_state.float()
     args = (values, steps, rates, keys, queries, skip, gate, step_bias, initial_state)
     if _gradients_wanted(*args):
-        return _SelectiveScan.apply(*args, bool(softplus), count, tokens, longest, sequences)
-    return _scan_forward(*args, bool(softplus), count, tokens, longest, offsets, False)[:2]
+        return _SelectiveScan.apply(*args, groups, int(softplus), count, tokens, longest, sequences)
+    return _scan_forward(*args, groups, int(softplus), count, tokens, longest, offsets, False)[:2]
 
 
 def selective_step(values: Tensor, steps: Tensor, rates: Tensor, keys: Tensor, queries: Tensor, state: Tensor, *,
@@ -497,7 +491,7 @@ def selective_step(values: Tensor, steps: Tensor, rates: Tensor, keys: Tensor, q
     """
     if values.ndim != 2:
         raise ValueError("values must be [B, C]")
-    rates, keys, queries, skip, step_bias = _scan_arguments(values, steps, rates, keys, queries, skip, gate, step_bias)
+    groups, rates, skip, step_bias = _scan_arguments(values, steps, rates, keys, queries, skip, gate, step_bias)
     b, (channels, n) = values.shape[0], rates.shape
     if state.shape != (b, channels, n):
         raise ValueError(f"state must be [{b}, {channels}, {n}]")
@@ -518,12 +512,10 @@ def selective_step(values: Tensor, steps: Tensor, rates: Tensor, keys: Tensor, q
     rates = rates.contiguous()
     skip = None if skip is None else skip.contiguous()
     step_bias = None if step_bias is None else step_bias.contiguous()
-    out = torch.empty(values.shape, device=values.device, dtype=values.dtype)
-    with torch.cuda.device(values.device):
-        rc = _capi.load().bssm_selective_step(
-            *flat, _DTYPES[values.dtype], rates.data_ptr(), _capi.ptr(skip), _capi.ptr(step_bias), int(softplus), b,
-            channels, n, keys.shape[-2], state.data_ptr(), out.data_ptr(), _stream(values.device))
-    _capi.check(rc, "bssm_selective_step")
+    out = _empty_like(values)
+    _capi.launch(values.device, "bssm_selective_step", *flat, _DTYPES[values.dtype], rates.data_ptr(),
+                 _capi.ptr(skip), _capi.ptr(step_bias), int(softplus), b, channels, n, groups, state.data_ptr(),
+                 out.data_ptr())
     del kept
     return out
 

@@ -12,10 +12,13 @@
 // loss and gradient NaN (nothing is read or written out of range).
 //
 // The traffic of the logits bounds it: read once, and the gradient written
-// once.  One CTA takes one row: a pass for the running maximum and sum, and,
-// where the gradient is wanted, a second one over a row that is then in L1 or
-// L2 (148 rows of 128 KB are 19 MB of its 126).  The K entries are corrected
-// afterwards, from the logits again rather than from the rounded gradient.
+// once.  A CTA takes a row (where rows are few, a cluster of CTAs takes one,
+// each a stretch of the vocabulary): a pass for the running maximum and sum,
+// and, where the gradient is wanted, a second one over logits that are then in
+// L2 (4 rows an SM of 64 to 128 KB are 38 to 76 MB of its 126).  The K entries
+// are corrected afterwards, from the logits again rather than from the rounded
+// gradient.  Sums are float32, taken in an order that sizes alone decide.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -27,8 +30,11 @@
 namespace bssm {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMaxTop = 1024;
+constexpr int kCounters = 148;       // partial counts of the rows with a teacher
+constexpr long kCountHere = 4096;    // entries up to which every CTA counts the rows itself
+constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct DistillArgs {
@@ -37,7 +43,7 @@ struct DistillArgs {
     int vocab, top, teacher_dtype, wide_indices;
     float temperature;
     int mean;
-    const int *count;        // rows with a teacher (mean)
+    int *counts;             // kCounters partial counts (mean, more than kCountHere entries)
     float *row_loss;         // forward
     float2 *row_stats;       // (maximum, sum of exp2((s - maximum) log2e / tau)); forward writes, backward reads
     void *grad;              // null: none
@@ -45,190 +51,303 @@ struct DistillArgs {
     int upstream_per_row;
 };
 
+__device__ __forceinline__ float exp2_unit(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// The maximum to subtract: where nothing but -inf was seen, any finite one.
+__device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
+
+// Running (maximum, sum) pairs joined: by the larger maximum.
+__device__ __forceinline__ float2 join(float2 a, float2 b, float scale) {
+    const float m = fmaxf(a.x, b.x), f = finite_max(m);
+    return make_float2(m, a.y * exp2_unit((a.x - f) * scale) + b.y * exp2_unit((b.x - f) * scale));
+}
+
 __device__ __forceinline__ long entry_of(const DistillArgs &a, long i) {
     return a.wide_indices ? static_cast<const long *>(a.indices)[i] : static_cast<const int *>(a.indices)[i];
 }
-
-// Reductions over the CTA; every thread gets the result.
-__device__ __forceinline__ float block_max(float v, float *scratch) {
-#pragma unroll
-    for (int o = 16; o > 0; o /= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) scratch[threadIdx.x / 32] = v;
-    __syncthreads();
-    v = scratch[threadIdx.x % (kThreads / 32)];
-#pragma unroll
-    for (int o = kThreads / 64; o > 0; o /= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
-__device__ __forceinline__ float block_sum(float v, float *scratch) {
-#pragma unroll
-    for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) scratch[threadIdx.x / 32] = v;
-    __syncthreads();
-    v = scratch[threadIdx.x % (kThreads / 32)];
-#pragma unroll
-    for (int o = kThreads / 64; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-
-// Rows with a teacher, added to *count: a warp per row.
-__device__ __forceinline__ bool has_entry(const DistillArgs &a, long i) {
+__device__ __forceinline__ bool is_entry(const DistillArgs &a, long i) {
     return entry_of(a, i) >= 0 && load_as_float(a.teacher, a.teacher_dtype, i) != -INFINITY;
 }
-__global__ void __launch_bounds__(256) distill_count(const DistillArgs a, int *count) {
-    const long warps = static_cast<long>(gridDim.x) * 8;
-    int mine = 0;
-    for (long r = static_cast<long>(blockIdx.x) * 8 + threadIdx.x / 32; r < a.rows; r += warps) {
+// Rows of first, first + step, ... with a teacher, by one warp.
+__device__ __forceinline__ int count_rows(const DistillArgs &a, long first, long step) {
+    int n = 0;
+    for (long r = first; r < a.rows; r += step) {
         bool any = false;
-        for (int k = threadIdx.x % 32; k < a.top && !any; k += 32) any = has_entry(a, r * a.top + k);
-        mine += __any_sync(0xffffffffu, any) ? 1 : 0;
+        for (int k = threadIdx.x % 32; k < a.top && !any; k += 32) any = is_entry(a, r * a.top + k);
+        n += __any_sync(0xffffffffu, any) ? 1 : 0;
     }
-    if (threadIdx.x % 32 == 0 && mine != 0) atomicAdd(count, mine);  // whole numbers: the order does not matter
+    return n;
+}
+__global__ void __launch_bounds__(kThreads) distill_count(const DistillArgs a) {
+    __shared__ int part[kWarps];
+    const int warp = threadIdx.x / 32;
+    const int n = count_rows(a, blockIdx.x * kWarps + warp, static_cast<long>(kCounters) * kWarps);
+    if (threadIdx.x % 32 == 0) part[warp] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int total = 0;
+        for (int w = 0; w < kWarps; ++w) total += part[w];
+        a.counts[blockIdx.x] = total;
+    }
+}
+// All rows with a teacher, in every thread of the CTA; `part` is its scratch.
+__device__ __forceinline__ int all_rows(const DistillArgs &a, int *part) {
+    int n = 0;
+    if (a.rows * a.top > kCountHere) {
+        for (int i = threadIdx.x % 32; i < kCounters; i += 32) n += a.counts[i];
+        return __reduce_add_sync(0xffffffffu, n);
+    }
+    n = count_rows(a, threadIdx.x / 32, kWarps);
+    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = n;
+    __syncthreads();
+    n = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) n += part[w];
+    return n;
 }
 
-// f(j, value) over a row's logits.  The row is walked in 16-byte vectors from
-// the first aligned element on, the ends element by element.
-template <typename T, typename F> __device__ __forceinline__ void for_row(const T *row, int n, F f) {
-    constexpr int VEC = 16 / sizeof(T);
-    const int head = min(n, static_cast<int>((16 - reinterpret_cast<uintptr_t>(row) % 16) % 16 / sizeof(T)));
-    const int vecs = (n - head) / VEC;
-    for (int j = threadIdx.x; j < head; j += kThreads) f(j, to_float(row[j]));
-    for (int i = threadIdx.x; i < vecs; i += kThreads) {
-        float v[VEC];
-        widen(load_packed<T, VEC>(row + head + i * VEC), v);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) f(head + i * VEC + e, v[e]);
+// A row's stretch [lo, hi): `head` single elements, `vecs` 16-byte vectors from
+// the first aligned address on, then single elements again.
+template <typename T> struct Stretch {
+    static constexpr int kVec = 16 / sizeof(T);
+    int lo, hi, body, vecs;
+    __device__ __forceinline__ Stretch(const T *row, int vocab, int rank, int ranks) {
+        // equal shares in whole vectors, counted from the row's first aligned element
+        const int head = min(vocab, static_cast<int>((16 - reinterpret_cast<uintptr_t>(row) % 16) % 16 / sizeof(T)));
+        const int all = (vocab - head) / kVec, share = (all + ranks - 1) / ranks;
+        const int first = min(all, rank * share), last = min(all, first + share);
+        body = head + first * kVec;
+        vecs = last - first;
+        lo = rank == 0 ? 0 : body;
+        hi = rank == ranks - 1 ? vocab : head + last * kVec;
     }
-    for (int j = head + vecs * VEC + threadIdx.x; j < n; j += kThreads) f(j, to_float(row[j]));
+    __device__ __forceinline__ int tail() const { return body + vecs * kVec; }
+};
+
+// One vector into a thread's running maximum and sum.
+template <int VEC> __device__ __forceinline__ void add_vector(const float (&v)[VEC], float scale, float &m, float &f,
+                                                              float2 &s) {
+    float top = fmaxf(v[0], v[1]);
+#pragma unroll
+    for (int e = 2; e < VEC; ++e) top = fmaxf(top, v[e]);
+    if (top > m) {
+        const float g = finite_max(top), by = m == -INFINITY ? 0.f : exp2_unit((m - g) * scale);
+        s = make_float2(s.x * by, s.y * by);
+        m = top;
+        f = g;
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; e += 2) {
+        const float2 x = __fmul2_rn(__fadd2_rn(make_float2(v[e], v[e + 1]), make_float2(-f, -f)),
+                                    make_float2(scale, scale));
+        s = __fadd2_rn(s, make_float2(exp2_unit(x.x), exp2_unit(x.y)));
+    }
 }
 
 // BACKWARD: the maximum and sum are the forward's.
-template <typename T, bool BACKWARD> __global__ void __launch_bounds__(kThreads) distill_rows(const DistillArgs a) {
-    __shared__ float scratch[kThreads / 32];
+template <typename T, bool BACKWARD> __global__ void __launch_bounds__(kThreads, 3) distill_rows(const DistillArgs a) {
+    constexpr int kVec = 16 / sizeof(T);
     __shared__ float p_s[kMaxTop];
-    __shared__ int i_s[kMaxTop];
-    __shared__ int bad_s;
-    const long r = blockIdx.x;
+    __shared__ __align__(16) int i_s[kMaxTop + 4];
+    __shared__ float2 stat_s[kWarps];
+    __shared__ float2 mine_s;  // this CTA's maximum and sum, read by its cluster
+    __shared__ int count_s[kWarps];
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = static_cast<int>(cluster.block_rank()), ranks = static_cast<int>(cluster.num_blocks());
+    const long r = blockIdx.x / ranks;
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const T *row = static_cast<const T *>(a.logits) + r * a.row_stride;
     T *grad = a.grad == nullptr ? nullptr : static_cast<T *>(a.grad) + r * a.vocab;
+    const Stretch<T> at(row, a.vocab, rank, ranks);
     const float scale = kLog2e / a.temperature;  // exponents in powers of two
 
-    // the teacher's softmax
-    if (threadIdx.x == 0) bad_s = 0;
-    __syncthreads();
-    float top = -INFINITY;
+    // the teacher's entries; -1 marks an empty one, -2 one past the vocabulary
     bool any = false;
-    for (int k = threadIdx.x; k < a.top; k += kThreads) {
+    for (int k = tid; k < a.top; k += kThreads) {
         const long e = entry_of(a, r * a.top + k);
-        float t = e < 0 ? -INFINITY : load_as_float(a.teacher, a.teacher_dtype, r * a.top + k);
-        if (e >= 0 && t != -INFINITY) any = true;
-        if (e >= a.vocab) bad_s = 1;
+        const float t = e < 0 ? -INFINITY : load_as_float(a.teacher, a.teacher_dtype, r * a.top + k);
+        any |= t != -INFINITY;
         p_s[k] = t;
-        i_s[k] = t == -INFINITY ? -1 : static_cast<int>(e >= a.vocab ? -1 : e);
-        top = fmaxf(top, t);
+        i_s[k] = t == -INFINITY ? -1 : e >= a.vocab ? -2 : static_cast<int>(e);
     }
-    any = __syncthreads_or(any);
-    if (!any) {  // no teacher
-        if (!BACKWARD && threadIdx.x == 0) a.row_loss[r] = 0.f;
+    if (tid < 4) i_s[a.top + tid] = -1;
+    if (!__syncthreads_or(any)) {  // no teacher
+        if (!BACKWARD && tid == 0 && rank == 0) a.row_loss[r] = 0.f;
         if (grad != nullptr)
-            for (int j = threadIdx.x; j < a.vocab; j += kThreads) grad[j] = from_float<T>(0.f);
-        return;
+            for (int j = at.lo + tid; j < at.hi; j += kThreads) grad[j] = from_float<T>(0.f);
+        return;  // every CTA of the cluster does
     }
-    top = block_max(top, scratch);
-    float part = 0.f;
-    for (int k = threadIdx.x; k < a.top; k += kThreads) {
-        const float e = p_s[k] == -INFINITY ? 0.f : exp2f((p_s[k] - top) * scale);
-        part += e;
-    }
-    const float total = block_sum(part, scratch);
 
-    float m, sum;
+    float2 stat;
     if (BACKWARD) {
-        m = a.row_stats[r].x;
-        sum = a.row_stats[r].y;
+        stat = a.row_stats[r];
     } else {
-        m = -INFINITY;
-        float s = 0.f;
-        bool nan = false;
-        for_row(row, a.vocab, [&](int, float v) {
-            if (v > m) {
-                s = s * exp2f((m - v) * scale);
-                m = v;
+        float m = -INFINITY, f = 0.f;
+        float2 s = make_float2(0.f, 0.f);
+        auto one = [&](int j) {
+            const float v[2] = {to_float(row[j]), -INFINITY};
+            add_vector<2>(v, scale, m, f, s);
+        };
+        for (int j = at.lo + tid; j < at.body; j += kThreads) one(j);
+        for (int j = at.tail() + tid; j < at.hi; j += kThreads) one(j);
+        const T *body = row + at.body;
+        int i = tid;
+        for (; i + 3 * kThreads < at.vecs; i += 4 * kThreads) {
+            Packed<T, kVec> p[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) p[u] = load_packed<T, kVec>(body + (i + u * kThreads) * kVec);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                float v[kVec];
+                widen(p[u], v);
+                add_vector<kVec>(v, scale, m, f, s);
             }
-            nan |= v != v;
-            s += m == -INFINITY ? 0.f : exp2f((v - m) * scale);
-        });
-        const float all = block_max(m, scratch);
-        s = m == -INFINITY ? 0.f : s * exp2f((m - all) * scale);
-        if (nan || all == INFINITY) s = NAN;
-        sum = block_sum(s, scratch);
-        m = all;
-        if (a.row_stats != nullptr && threadIdx.x == 0) a.row_stats[r] = make_float2(m, sum);
+        }
+        for (; i < at.vecs; i += kThreads) {
+            float v[kVec];
+            widen(load_packed<T, kVec>(body + i * kVec), v);
+            add_vector<kVec>(v, scale, m, f, s);
+        }
+        stat = make_float2(m, s.x + s.y);
+        float2 all = make_float2(warp_max(m), 0.f);
+        all.y = warp_sum(stat.y * exp2_unit((m - finite_max(all.x)) * scale));
+        if (lane == 0) stat_s[warp] = all;
+        __syncthreads();
+        stat = stat_s[0];
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) stat = join(stat, stat_s[w], scale);
+        if (ranks > 1) {
+            if (tid == 0) mine_s = stat;
+            cluster.sync();
+            stat = *cluster.map_shared_rank(&mine_s, 0);
+            for (int w = 1; w < ranks; ++w) stat = join(stat, *cluster.map_shared_rank(&mine_s, w), scale);
+            cluster.sync();  // no CTA leaves while another still reads its pair
+        }
+        if (a.row_stats != nullptr && tid == 0 && rank == 0) a.row_stats[r] = stat;
     }
-    const float bad = bad_s ? NAN : 0.f;
-    const float inverse = 1.f / sum + bad;
+    // a row of -inf alone has no distribution: m is -inf and what follows is NaN
+    const float m = stat.x, sum = stat.y;
+    // the teacher's softmax, in every warp
+    float top = -INFINITY, total = 0.f;
+    bool bad = false;
+    for (int k = lane; k < a.top; k += 32) {
+        top = fmaxf(top, p_s[k]);
+        bad |= i_s[k] == -2;
+    }
+    const float poison = __any_sync(0xffffffffu, bad) ? NAN : 0.f, inverse = 1.f / sum + poison;
+    top = warp_max(top);
+    for (int k = lane; k < a.top; k += 32) total += exp2f((p_s[k] - top) * scale);
+    total = warp_sum(total);
 
-    if (!BACKWARD) {
+    if (!BACKWARD && warp == 0 && rank == 0) {
         const float log_total = log2f(total), log_sum = log2f(sum);
         float loss = 0.f;
-        for (int k = threadIdx.x; k < a.top; k += kThreads) {
+        for (int k = lane; k < a.top; k += 32) {
             if (i_s[k] < 0) continue;
             const float lp = (p_s[k] - top) * scale - log_total, p = exp2f(lp);
             const float lq = (to_float(row[i_s[k]]) - m) * scale - log_sum;
             if (p != 0.f) loss = fmaf(p, lp - lq, loss);
         }
-        loss = block_sum(loss, scratch);
-        if (threadIdx.x == 0) a.row_loss[r] = loss * kLn2 * a.temperature * a.temperature + bad + (sum != sum ? NAN : 0.f);
+        loss = warp_sum(loss);
+        if (lane == 0)
+            a.row_loss[r] = loss * kLn2 * a.temperature * a.temperature + poison + (sum != sum ? NAN : 0.f);
     }
     if (grad == nullptr) return;
     float weight = a.temperature;
     if (a.upstream != nullptr) weight *= a.upstream[a.upstream_per_row ? r : 0];
-    if (a.mean) weight /= static_cast<float>(max(1, *a.count));
-    if ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(grad)) % 16 == 0) {
-        constexpr int VEC = 16 / sizeof(T);
-        const int head = min(a.vocab, static_cast<int>((16 - reinterpret_cast<uintptr_t>(row) % 16) % 16 / sizeof(T)));
-        const int vecs = (a.vocab - head) / VEC;
-        auto one = [&](int j) { grad[j] = from_float<T>(weight * (exp2f((to_float(row[j]) - m) * scale) * inverse)); };
-        for (int j = threadIdx.x; j < head; j += kThreads) one(j);
-        for (int i = threadIdx.x; i < vecs; i += kThreads) {
-            float v[VEC];
-            widen(load_packed<T, VEC>(row + head + i * VEC), v);
+    if (a.mean) weight /= static_cast<float>(max(1, all_rows(a, count_s)));
+    const float factor = weight * inverse;
+    auto one = [&](int j) { grad[j] = from_float<T>(exp2_unit((to_float(row[j]) - m) * scale) * factor); };
+    auto eight = [&](const Packed<T, kVec> &p, float (&v)[kVec]) {
+        widen(p, v);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] = weight * (exp2f((v[e] - m) * scale) * inverse);
-            store_packed<T, VEC>(grad + head + i * VEC, v);
+        for (int e = 0; e < kVec; e += 2) {
+            const float2 x = __fmul2_rn(__fadd2_rn(make_float2(v[e], v[e + 1]), make_float2(-m, -m)),
+                                        make_float2(scale, scale));
+            const float2 g = __fmul2_rn(make_float2(exp2_unit(x.x), exp2_unit(x.y)), make_float2(factor, factor));
+            v[e] = g.x;
+            v[e + 1] = g.y;
         }
-        for (int j = head + vecs * VEC + threadIdx.x; j < a.vocab; j += kThreads) one(j);
-    } else {
-        for_row(row, a.vocab, [&](int j, float v) {
-            grad[j] = from_float<T>(weight * (exp2f((v - m) * scale) * inverse));
-        });
+    };
+    if ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(grad)) % 16 == 0) {
+        for (int j = at.lo + tid; j < at.body; j += kThreads) one(j);
+        for (int j = at.tail() + tid; j < at.hi; j += kThreads) one(j);
+        const T *body = row + at.body;
+        T *out = grad + at.body;
+        int i = tid;
+        for (; i + 3 * kThreads < at.vecs; i += 4 * kThreads) {
+            Packed<T, kVec> p[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) p[u] = load_packed<T, kVec>(body + (i + u * kThreads) * kVec);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                float v[kVec];
+                eight(p[u], v);
+                store_packed<T, kVec>(out + (i + u * kThreads) * kVec, v);
+            }
+        }
+        for (; i < at.vecs; i += kThreads) {
+            float v[kVec];
+            eight(load_packed<T, kVec>(body + i * kVec), v);
+            store_packed<T, kVec>(out + i * kVec, v);
+        }
+    } else {  // rows of logits and gradient fall differently on 16 bytes
+        for (int j = at.lo + tid; j < at.hi; j += kThreads) one(j);
     }
     __syncthreads();
     // the entries the teacher names: q - p, the p of an entry named twice added up
-    for (int k = threadIdx.x; k < a.top; k += kThreads) {
+    const float per = 1.f / total;
+    for (int k = tid; k < a.top; k += kThreads) {
         const int j = i_s[k];
-        if (j < 0) continue;
-        float p = 0.f;
-        bool first = true;
-        for (int o = 0; o < a.top; ++o) {
-            if (i_s[o] != j) continue;
-            if (o < k) first = false;
-            p += exp2f((p_s[o] - top) * scale) / total;
+        if (j < at.lo || j >= at.hi) continue;
+        int same = 0;
+        for (int o = 0; o < a.top; o += 4) {
+            const int4 i = *reinterpret_cast<const int4 *>(&i_s[o]);
+            same += (i.x == j) + (i.y == j) + (i.z == j) + (i.w == j);
         }
-        if (first) grad[j] = from_float<T>(weight * (exp2f((to_float(row[j]) - m) * scale) * inverse - p));
+        float p = exp2f((p_s[k] - top) * scale) * per;
+        if (same > 1) {
+            bool first = true;
+            p = 0.f;
+            for (int o = 0; o < a.top; ++o) {
+                if (i_s[o] != j) continue;
+                first &= o >= k;
+                p += exp2f((p_s[o] - top) * scale) * per;
+            }
+            if (!first) continue;
+        }
+        grad[j] = from_float<T>(weight * (exp2_unit((to_float(row[j]) - m) * scale) * inverse - p));
     }
 }
 
 // The rows' losses added in a fixed order, and divided by the rows counted.
-__global__ void __launch_bounds__(kThreads) distill_total(const float *row_loss, long rows, int mean, const int *count,
-                                                          float *loss) {
-    __shared__ float scratch[kThreads / 32];
+__global__ void __launch_bounds__(kThreads) distill_total(const DistillArgs a, float *loss) {
+    __shared__ float part[kWarps];
+    __shared__ int count_s[kWarps];
     float v = 0.f;
-    for (long r = threadIdx.x; r < rows; r += kThreads) v += row_loss[r];
-    v = block_sum(v, scratch);
-    if (threadIdx.x == 0) *loss = mean ? v / static_cast<float>(max(1, *count)) : v;
+    for (long r = threadIdx.x; r < a.rows; r += kThreads) v += a.row_loss[r];
+    v = warp_sum(v);
+    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = v;
+    __syncthreads();
+    const int n = a.mean ? all_rows(a, count_s) : 1;
+    if (threadIdx.x != 0) return;
+    v = 0.f;
+    for (int w = 0; w < kWarps; ++w) v += part[w];
+    *loss = v / static_cast<float>(max(1, n));
 }
 
 // grad *= *factor, nothing at all where it is 1 (the loss was the end of the graph).
@@ -240,9 +359,22 @@ template <typename T> __global__ void __launch_bounds__(256) distill_scale(T *gr
 }
 
 template <typename T> int launch_rows(const DistillArgs &a, bool backward, cudaStream_t st) {
-    const unsigned grid = static_cast<unsigned>(a.rows);
-    if (backward) distill_rows<T, true><<<grid, kThreads, 0, st>>>(a);
-    else distill_rows<T, false><<<grid, kThreads, 0, st>>>(a);
+    // Rows alone fill the SMs from 148 on.  Fewer are split, up to a cluster of 8 and 4,096 logits a CTA.
+    int ranks = 1;
+    while (ranks < kMaxCluster && a.rows * ranks * 2 <= 296 && a.vocab / (ranks * 2) >= 4096) ranks *= 2;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>(a.rows * ranks));
+    config.blockDim = dim3(kThreads);
+    config.stream = st;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = static_cast<unsigned>(ranks);
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    const cudaError_t e = backward ? cudaLaunchKernelEx(&config, distill_rows<T, true>, a)
+                                   : cudaLaunchKernelEx(&config, distill_rows<T, false>, a);
+    if (e != cudaSuccess) return fail(BSSM_ERR_CUDA, "distillation: %s", cudaGetErrorString(e));
     return check_launch("distillation");
 }
 int launch_rows(int dtype, const DistillArgs &a, bool backward, cudaStream_t st) {
@@ -259,53 +391,49 @@ int check_distill(const char *what, int dtype, long rows, int vocab, long row_st
         return fail(BSSM_ERR_UNSUPPORTED, "%s: unknown dtype", what);
     if (top < 1 || top > kMaxTop)
         return fail(BSSM_ERR_UNSUPPORTED, "%s: %d teacher logits a row (1 to %d are built)", what, top, kMaxTop);
-    if (rows < 0 || rows > 0x7fffffffL || vocab < 1 || (rows > 1 && row_stride < vocab) || !(temperature > 0.f) ||
+    if (rows < 0 || rows > 0x7fffffffL / 8 || vocab < 1 || (rows > 1 && row_stride < vocab) || !(temperature > 0.f) ||
         !(temperature < INFINITY))
         return fail(BSSM_ERR_INVALID, "%s: bad sizes or temperature", what);
     return BSSM_OK;
 }
 
-int count_rows(const DistillArgs &a, int *count, cudaStream_t st) {
-    if (cudaError_t e = cudaMemsetAsync(count, 0, sizeof(int), st))
-        return fail(BSSM_ERR_CUDA, "distillation: %s", cudaGetErrorString(e));
-    const long blocks = (a.rows + 7) / 8;
-    if (blocks > 0) distill_count<<<static_cast<unsigned>(blocks < 592 ? blocks : 592), 256, 0, st>>>(a, count);
-    return check_launch("distillation");
-}
-
 }  // namespace
 }  // namespace bssm
+
+extern "C" int bssm_distillation_counters(void) { return bssm::kCounters; }
 
 extern "C" int bssm_distillation(const void *logits, int dtype, long rows, int vocab, long row_stride,
                                  const void *teacher, int teacher_dtype, const void *indices, int index_bytes, int top,
                                  float temperature, int mean, float *row_loss, float *row_stats, float *loss,
-                                 int *count, void *grad, void *stream) {
+                                 int *counts, void *grad, void *stream) {
     using namespace bssm;
     if (int rc = check_distill("distillation", dtype, rows, vocab, row_stride, top, teacher_dtype, index_bytes,
                                temperature))
         return rc;
     if ((rows > 0 && (logits == nullptr || teacher == nullptr || indices == nullptr || row_loss == nullptr)) ||
-        (mean && count == nullptr))
+        (mean && counts == nullptr))
         return fail(BSSM_ERR_INVALID, "distillation: null pointer");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     DistillArgs a{};
     a.logits = logits; a.teacher = teacher; a.indices = indices; a.rows = rows; a.row_stride = row_stride;
     a.vocab = vocab; a.top = top; a.teacher_dtype = teacher_dtype; a.wide_indices = index_bytes == 8;
-    a.temperature = temperature; a.mean = mean; a.count = count; a.row_loss = row_loss;
+    a.temperature = temperature; a.mean = mean; a.counts = counts; a.row_loss = row_loss;
     a.row_stats = reinterpret_cast<float2 *>(row_stats); a.grad = grad;
-    if (mean)
-        if (int rc = count_rows(a, count, st)) return rc;
+    if (mean && rows * top > kCountHere) {
+        distill_count<<<kCounters, kThreads, 0, st>>>(a);
+        if (int rc = check_launch("distillation")) return rc;
+    }
     if (rows > 0)
         if (int rc = launch_rows(dtype, a, false, st)) return rc;
     if (loss == nullptr) return BSSM_OK;
-    distill_total<<<1, kThreads, 0, st>>>(row_loss, rows, mean, count, loss);
+    distill_total<<<1, kThreads, 0, st>>>(a, loss);
     return check_launch("distillation");
 }
 
 extern "C" int bssm_distillation_backward(const void *logits, int dtype, long rows, int vocab, long row_stride,
                                           const void *teacher, int teacher_dtype, const void *indices, int index_bytes,
                                           int top, float temperature, int mean, const float *row_stats,
-                                          const int *count, const float *upstream, int upstream_per_row, void *grad,
+                                          const int *counts, const float *upstream, int upstream_per_row, void *grad,
                                           void *stream) {
     using namespace bssm;
     if (int rc = check_distill("distillation_backward", dtype, rows, vocab, row_stride, top, teacher_dtype, index_bytes,
@@ -313,13 +441,13 @@ extern "C" int bssm_distillation_backward(const void *logits, int dtype, long ro
         return rc;
     if ((rows > 0 && (logits == nullptr || teacher == nullptr || indices == nullptr || row_stats == nullptr ||
                       grad == nullptr)) ||
-        (mean && count == nullptr))
+        (mean && counts == nullptr))
         return fail(BSSM_ERR_INVALID, "distillation_backward: null pointer");
     if (rows == 0) return BSSM_OK;
     DistillArgs a{};
     a.logits = logits; a.teacher = teacher; a.indices = indices; a.rows = rows; a.row_stride = row_stride;
     a.vocab = vocab; a.top = top; a.teacher_dtype = teacher_dtype; a.wide_indices = index_bytes == 8;
-    a.temperature = temperature; a.mean = mean; a.count = count;
+    a.temperature = temperature; a.mean = mean; a.counts = const_cast<int *>(counts);
     a.row_stats = reinterpret_cast<float2 *>(const_cast<float *>(row_stats));
     a.grad = grad; a.upstream = upstream; a.upstream_per_row = upstream_per_row;
     return launch_rows(dtype, a, true, static_cast<cudaStream_t>(stream));

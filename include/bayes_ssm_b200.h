@@ -509,17 +509,19 @@ int bssm_selective_step(const void *values, long value_stride, const void *steps
  * indices (index_bytes 4 or 8) are [rows][top].
  * row_stats (two floats a row) is what the backward needs.  loss (may be
  * null) receives the sum of row_loss, divided, with mean != 0, by the number
- * of rows that have a teacher, which is left in *count.  grad (may be null)
+ * of rows that have a teacher; for a mean, counts (bssm_distillation_counters()
+ * ints) is scratch that the backward reads again.  grad (may be null)
  * [rows][vocab] receives the gradient of that loss; the backward writes it
  * times *upstream, or times upstream[row].
  * bssm_distillation_scale multiplies n values by the device float *factor.
  */
+int bssm_distillation_counters(void);
 int bssm_distillation(const void *logits, int dtype, long rows, int vocab, long row_stride, const void *teacher,
                       int teacher_dtype, const void *indices, int index_bytes, int top, float temperature, int mean,
-                      float *row_loss, float *row_stats, float *loss, int *count, void *grad, void *stream);
+                      float *row_loss, float *row_stats, float *loss, int *counts, void *grad, void *stream);
 int bssm_distillation_backward(const void *logits, int dtype, long rows, int vocab, long row_stride,
                                const void *teacher, int teacher_dtype, const void *indices, int index_bytes, int top,
-                               float temperature, int mean, const float *row_stats, const int *count,
+                               float temperature, int mean, const float *row_stats, const int *counts,
                                const float *upstream, int upstream_per_row, void *grad, void *stream);
 int bssm_distillation_scale(void *grad, int dtype, long n, const float *factor, void *stream);
 
