@@ -11,12 +11,13 @@
 // Bayesian mixer's features.)
 //
 // All of it is bound by the rows' traffic: x in and y out, or x and dy in and
-// dx out.  A thread owns VEC adjacent channels (16 bytes where the rows allow
-// it) and walks a run of tokens with the window in registers, four tokens'
-// loads in flight, so each row is read once apart from W - 1 rows per run.
+// dx out.  A thread owns VEC adjacent channels (2 where the rows allow
+// it) and walks a run of tokens with the window in registers, the next four
+// tokens' loads in flight, so each row is read once apart from W - 1 rows per run.
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "bayes_ssm_b200.h"
 #include "bssm_internal.h"
@@ -38,14 +39,44 @@ struct ConvArgs {
     long run, runs;
 };
 
+template <typename TW, int VEC, int W>
+__device__ __forceinline__ void load_taps_of(const TW *weight, long c, float (&w)[W][VEC]) {
+    constexpr int kCount = VEC * W;
+    float v[kCount];
+    constexpr int kStep = 16 / sizeof(TW) < kCount ? 16 / sizeof(TW) : kCount;
+    const TW *p = weight + c * W;
+    if (kCount % kStep == 0 && (kStep & (kStep - 1)) == 0 && reinterpret_cast<uintptr_t>(p) % (kStep * sizeof(TW)) == 0) {
+#pragma unroll
+        for (int o = 0; o < kCount; o += kStep) {
+            const Packed<TW, kStep> q = load_packed<TW, kStep>(p + o);
+#pragma unroll
+            for (int e = 0; e < kStep; ++e) v[o + e] = to_float(q.e[e]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < kCount; ++e) v[e] = to_float(p[e]);
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+#pragma unroll
+        for (int j = 0; j < W; ++j) w[j][i] = v[i * W + j];
+}
+template <typename TW, int VEC> __device__ __forceinline__ void load_bias_of(const TW *bias, long c, float (&b)[VEC]) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) b[i] = to_float(bias[c + i]);
+}
+// The type is tested once, so that the loads go out together.
 template <int VEC, int W>
 __device__ __forceinline__ void load_taps(const ConvArgs &a, long c, float (&w)[W][VEC], float (&b)[VEC]) {
+    if (a.w_dtype == BSSM_F32) load_taps_of(static_cast<const float *>(a.weight), c, w);
+    else if (a.w_dtype == BSSM_BF16) load_taps_of(static_cast<const __nv_bfloat16 *>(a.weight), c, w);
+    else load_taps_of(static_cast<const __half *>(a.weight), c, w);
+    if (a.bias == nullptr) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-#pragma unroll
-        for (int j = 0; j < W; ++j) w[j][i] = load_as_float(a.weight, a.w_dtype, (c + i) * W + j);
-        b[i] = a.bias == nullptr ? 0.f : load_as_float(a.bias, a.b_dtype, c + i);
-    }
+        for (int i = 0; i < VEC; ++i) b[i] = 0.f;
+    } else if (a.b_dtype == BSSM_F32) load_bias_of(static_cast<const float *>(a.bias), c, b);
+    else if (a.b_dtype == BSSM_BF16) load_bias_of(static_cast<const __nv_bfloat16 *>(a.bias), c, b);
+    else load_bias_of(static_cast<const __half *>(a.bias), c, b);
 }
 
 // The input at row `g` of sequence s, whose first row is `first`: a row before
@@ -63,18 +94,39 @@ __device__ __forceinline__ void load_input(const ConvArgs &a, long s, long first
     }
 }
 
+// acc += a b, two channels an instruction
+template <int VEC>
+__device__ __forceinline__ void fma_to(float (&acc)[VEC], const float (&a)[VEC], const float (&b)[VEC]) {
+    if constexpr (VEC == 1) {
+        acc[0] = fmaf(a[0], b[0], acc[0]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2) {
+            const float2 r = __ffma2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]),
+                                        make_float2(acc[i], acc[i + 1]));
+            acc[i] = r.x;
+            acc[i + 1] = r.y;
+        }
+    }
+}
+
 // u of one token from the window (the W - 1 inputs before it) and its own input
 template <int VEC, int W>
 __device__ __forceinline__ void preactivation(const float (&w)[W][VEC], const float (&b)[VEC],
                                               const float (&win)[W - 1][VEC], const float (&x)[VEC],
                                               float (&u)[VEC]) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-        float v = b[i];
+    for (int i = 0; i < VEC; ++i) u[i] = b[i];
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) v = fmaf(w[j][i], win[j][i], v);
-        u[i] = fmaf(w[W - 1][i], x[i], v);
-    }
+    for (int j = 0; j < W - 1; ++j) fma_to(u, w[j], win[j]);
+    fma_to(u, w[W - 1], x);
+}
+
+// 1 / (1 + exp(-u)).  Rows of 16 bits take the short form, whose exponent is
+// rounded first (|u| 2^-24 of the result, far below the rows' own rounding).
+template <typename T> __device__ __forceinline__ float sigmoid_for(float u) {
+    if (sizeof(T) == 4) return sigmoid_f(u);
+    return __fdividef(1.f, 1.f + __expf(-u));
 }
 
 template <int VEC, int ROWS> __device__ __forceinline__ void slide(float (&win)[ROWS][VEC], const float (&x)[VEC]) {
@@ -86,14 +138,14 @@ template <int VEC, int ROWS> __device__ __forceinline__ void slide(float (&win)[
     for (int i = 0; i < VEC; ++i) win[ROWS - 1][i] = x[i];
 }
 
-__device__ __forceinline__ float silu_slope(float u) {
-    const float s = sigmoid_f(u);
+template <typename T> __device__ __forceinline__ float silu_slope(float u) {
+    const float s = sigmoid_for<T>(u);
     return s * fmaf(u, 1.f - s, 1.f);
 }
 
 // Threads 0 .. nvec * runs - 1 walk one run of tokens each; the threads after
 // them write the states after the last tokens, one state row each.
-template <typename T, int VEC, int W> __global__ void __launch_bounds__(kThreads) conv_forward(const ConvArgs a) {
+template <typename T, int VEC, int W> __global__ void __launch_bounds__(kThreads, 4) conv_forward(const ConvArgs a) {
     const long nvec = a.channels / VEC;
     const long id = static_cast<long>(blockIdx.x) * kThreads + threadIdx.x;
     const long c = id % nvec * VEC, r = id / nvec;
@@ -116,7 +168,7 @@ template <typename T, int VEC, int W> __global__ void __launch_bounds__(kThreads
         preactivation<VEC, W>(w, b, win, v, u);
         if (a.silu) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) u[i] *= sigmoid_f(u[i]);
+            for (int i = 0; i < VEC; ++i) u[i] *= sigmoid_for<T>(u[i]);
         }
         store_packed<T, VEC>(y + g * a.channels, u);
     };
@@ -129,14 +181,22 @@ template <typename T, int VEC, int W> __global__ void __launch_bounds__(kThreads
         float win[W - 1][VEC];
 #pragma unroll
         for (int j = 0; j < W - 1; ++j) load_input<T, VEC, W>(a, s, first, g - (W - 1) + j, c, win[j]);
-        for (; g + kAhead <= last; g += kAhead) {
-            Packed<T, VEC> p[kAhead];
+        Packed<T, VEC> p[kAhead];
+        auto load = [&](long t) {
+            if (t + kAhead > last) return;
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) p[k] = load_packed<T, VEC>(x + (g + k) * a.row_stride);
+            for (int k = 0; k < kAhead; ++k) p[k] = load_packed<T, VEC>(x + (t + k) * a.row_stride);
+        };
+        load(g);
+        for (; g + kAhead <= last; g += kAhead) {
+            Packed<T, VEC> now[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) now[k] = p[k];
+            load(g + kAhead);
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
                 float v[VEC];
-                widen(p[k], v);
+                widen(now[k], v);
                 emit(g + k, win, v);
                 slide<VEC, W - 1>(win, v);
             }
@@ -158,7 +218,7 @@ template <typename T, int VEC, int W> __global__ void __launch_bounds__(kThreads
 // tokens past its run for the du they need; the run's dw and db stay in
 // registers and are written as one row of `partial` [runs][W + 1][channels],
 // which sum_rows adds up in a fixed order.
-template <typename T, int VEC, int W> __global__ void __launch_bounds__(kThreads) conv_backward(const ConvArgs a) {
+template <typename T, int VEC, int W> __global__ void __launch_bounds__(kThreads, 3) conv_backward(const ConvArgs a) {
     const long nvec = a.channels / VEC;
     const long id = static_cast<long>(blockIdx.x) * kThreads + threadIdx.x;
     const long c = id % nvec * VEC, r = id / nvec;
@@ -184,7 +244,7 @@ template <typename T, int VEC, int W> __global__ void __launch_bounds__(kThreads
             widen(load_packed<T, VEC>(gy + (first + t) * a.channels), dy);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                const float du = a.silu ? dy[i] * silu_slope(u[i]) : dy[i];
+                const float du = a.silu ? dy[i] * silu_slope<T>(u[i]) : dy[i];
                 float tap = 0.f;
 #pragma unroll
                 for (int j = 0; j < W - 1; ++j) tap = j == m - t ? w[j][i] : tap;
@@ -219,59 +279,74 @@ template <typename T, int VEC, int W> __global__ void __launch_bounds__(kThreads
 #pragma unroll
             for (int i = 0; i < VEC; ++i) past[j][i] = 0.f;
         }
-        const long steps = hi - lo + W - 1;
-        for (long k0 = 0; k0 < steps; k0 += kAhead) {
+        // Token t: its du, the run's dw and db where t is the run's, and dx of W - 1 tokens before.  INNER: all of
+        // these are the run's and no final state's gradient comes in.
+        auto advance = [&](auto inner, long t, const float (&v)[VEC], float (&du)[VEC]) {
+            constexpr bool kInner = decltype(inner)::value;
+            if (a.silu) {
+                float u[VEC];
+                preactivation<VEC, W>(w, b, win, v, u);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) du[i] *= silu_slope<T>(u[i]);
+            }
+            if (kInner || t < hi) {
+#pragma unroll
+                for (int j = 0; j < W - 1; ++j) fma_to(dw[j], du, win[j]);
+                fma_to(dw[W - 1], du, v);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) db[i] += du[i];
+            }
+            const long out = t - (W - 1);
+            if (kInner || out >= lo) {
+                float o[VEC] = {};
+                const long kept = out - (last - (W - 1));
+                if (!kInner && gs != nullptr && kept >= 0)
+                    widen(load_packed<T, VEC>(gs + (s * (W - 1) + kept) * a.channels + c), o);
+                fma_to(o, w[0], du);
+#pragma unroll
+                for (int j = 0; j < W - 1; ++j) fma_to(o, w[W - 1 - j], past[j]);
+                store_packed<T, VEC>(gx + out * a.channels, o);
+            }
+            slide<VEC, W - 1>(win, v);
+            slide<VEC, W - 1>(past, du);
+        };
+        auto edge = [&](long t) {  // a token at either end of the piece, or past the sequence's
+            float v[VEC] = {}, du[VEC] = {};
+            if (t < last) {
+                widen(load_packed<T, VEC>(x + t * a.row_stride), v);
+                widen(load_packed<T, VEC>(gy + t * a.channels), du);
+            }
+            advance(std::false_type{}, t, v, du);
+        };
+        long t = lo;
+        for (; t < lo + W - 1 && t < hi + W - 1; ++t) edge(t);
+        Packed<T, VEC> next_x[kAhead], next_g[kAhead];
+        auto load = [&](long from) {
+            if (from + kAhead > hi) return;
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                next_x[k] = load_packed<T, VEC>(x + (from + k) * a.row_stride);
+                next_g[k] = load_packed<T, VEC>(gy + (from + k) * a.channels);
+            }
+        };
+        load(t);
+        for (; t + kAhead <= hi; t += kAhead) {
             Packed<T, VEC> px[kAhead], pg[kAhead];
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
-                const long t = lo + k0 + k;
-                if (k0 + k < steps && t < last) {
-                    px[k] = load_packed<T, VEC>(x + t * a.row_stride);
-                    pg[k] = load_packed<T, VEC>(gy + t * a.channels);
-                }
+                px[k] = next_x[k];
+                pg[k] = next_g[k];
             }
+            load(t + kAhead);
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
-                const long t = lo + k0 + k;
-                if (k0 + k >= steps) break;
-                float v[VEC] = {}, du[VEC] = {};
-                if (t < last) {
-                    float u[VEC];
-                    widen(px[k], v);
-                    widen(pg[k], du);
-                    if (a.silu) {
-                        preactivation<VEC, W>(w, b, win, v, u);
-#pragma unroll
-                        for (int i = 0; i < VEC; ++i) du[i] *= silu_slope(u[i]);
-                    }
-                    if (t < hi) {
-#pragma unroll
-                        for (int i = 0; i < VEC; ++i) {
-                            db[i] += du[i];
-#pragma unroll
-                            for (int j = 0; j < W - 1; ++j) dw[j][i] = fmaf(du[i], win[j][i], dw[j][i]);
-                            dw[W - 1][i] = fmaf(du[i], v[i], dw[W - 1][i]);
-                        }
-                    }
-                }
-                const long out = t - (W - 1);
-                if (out >= lo) {
-                    float o[VEC] = {};
-                    const long kept = out - (last - (W - 1));
-                    if (gs != nullptr && kept >= 0)
-                        widen(load_packed<T, VEC>(gs + (s * (W - 1) + kept) * a.channels + c), o);
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) {
-#pragma unroll
-                        for (int j = 0; j < W - 1; ++j) o[i] = fmaf(w[W - 1 - j][i], past[j][i], o[i]);
-                        o[i] = fmaf(w[0][i], du[i], o[i]);
-                    }
-                    store_packed<T, VEC>(gx + out * a.channels, o);
-                }
-                slide<VEC, W - 1>(win, v);
-                slide<VEC, W - 1>(past, du);
+                float v[VEC], du[VEC];
+                widen(px[k], v);
+                widen(pg[k], du);
+                advance(std::true_type{}, t + k, v, du);
             }
         }
+        for (; t < hi + W - 1; ++t) edge(t);
         g = hi;
     }
     float *p = a.partial + r * (W + 1) * a.channels + c;
@@ -324,7 +399,7 @@ template <typename T, int VEC, int W> __global__ void __launch_bounds__(kThreads
     preactivation<VEC, W>(w, b, win, v, u);
     if (a.silu) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) u[i] *= sigmoid_f(u[i]);
+        for (int i = 0; i < VEC; ++i) u[i] *= sigmoid_for<T>(u[i]);
     }
     store_packed<T, VEC>(static_cast<T *>(a.y) + s * a.channels + c, u);
 #pragma unroll
@@ -354,7 +429,9 @@ template <typename T, int VEC> int pick_taps(ConvKind kind, int taps, const Conv
     }
 }
 
-// The widest vector that the channel count, the row stride and every address allow.
+// Two channels a thread where the channel count, the row stride and every
+// address allow it.  Four or eight would make 8- or 16-byte loads, but taps,
+// windows and loads in flight then leave few warps an SM or spill.
 template <typename T> int pick_vector(ConvKind kind, int taps, const ConvArgs &a, cudaStream_t st) {
     uintptr_t bits = 0;
     for (const void *p : {a.x, a.state0, a.grad_y, a.grad_state1, static_cast<const void *>(a.y),
@@ -362,10 +439,7 @@ template <typename T> int pick_vector(ConvKind kind, int taps, const ConvArgs &a
                           static_cast<const void *>(a.grad_state0)})
         bits |= reinterpret_cast<uintptr_t>(p);
     bits |= static_cast<uintptr_t>(a.channels) * sizeof(T) | static_cast<uintptr_t>(a.row_stride) * sizeof(T);
-    constexpr int widest = 16 / sizeof(T);
-    if (bits % 16 == 0) return pick_taps<T, widest>(kind, taps, a, st);
-    if (bits % 8 == 0) return pick_taps<T, widest / 2>(kind, taps, a, st);
-    if (sizeof(T) == 2 && bits % 4 == 0) return pick_taps<T, 2>(kind, taps, a, st);
+    if (bits % (2 * sizeof(T)) == 0) return pick_taps<T, 2>(kind, taps, a, st);
     return pick_taps<T, 1>(kind, taps, a, st);
 }
 
@@ -420,7 +494,7 @@ extern "C" int bssm_causal_conv(const void *x, int dtype, long row_stride, long 
     a.x = x; a.weight = weight; a.bias = bias; a.state0 = state0; a.y = y; a.state1 = state1;
     a.row_stride = row_stride; a.seq = make_sequences(offsets, sequences, tokens);
     a.channels = channels; a.w_dtype = weight_dtype; a.b_dtype = bias_dtype; a.silu = silu;
-    a.run = run_length(tokens, channels, 16);
+    a.run = run_length(tokens, channels, 32);
     a.runs = (tokens + a.run - 1) / a.run;
     return pick_type(kForward, dtype, taps, a, static_cast<cudaStream_t>(stream));
 }

@@ -41,7 +41,7 @@ __host__ __device__ constexpr int io_dtype_bytes(int dtype) { return dtype == BS
 
 // VEC consecutive elements as float32, in one access when VEC * sizeof(T) <= 16
 // (the address must then be a multiple of that), else in 16-byte accesses.
-template <typename T, int VEC> struct alignas(VEC * sizeof(T) < 16 ? VEC * sizeof(T) : 16) Packed {
+template <typename T, int VEC> struct alignas((VEC & (VEC - 1)) != 0 ? sizeof(T) : VEC * sizeof(T) < 16 ? VEC * sizeof(T) : 16) Packed {
     T e[VEC];
 };
 template <typename T, int VEC> __device__ __forceinline__ void widen(const Packed<T, VEC> &p, float (&o)[VEC]) {
