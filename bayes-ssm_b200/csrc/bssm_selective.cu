@@ -13,18 +13,20 @@
 //   dq_t = sum_c dr h,  dk_t = sum_c g d x,  dx = skip dr + d (g.k)
 //   dd   = sum_n g (A a h_{t-1} + x k),  dA = sum_t g d a h_{t-1},  a = exp(d A)
 //
-// Work split.  A lane holds 4 states of a channel and LPC = ceil(N / 4) lanes
-// (a power of two, 1..16) hold the channel, so the sums over N take log2(LPC)
+// Work split.  A lane holds 2 states of a channel and LPC = ceil(N / 2) lanes
+// (a power of two, 1..32) hold the channel, so the sums over N take log2(LPC)
 // exchanges and a warp advances 32 / LPC channels; tokens are walked in order.
-// A CTA of 8 warps holds CH adjacent channels of one group and one sequence.
-// Its threads first turn a tile of tokens into d, d x (and dr) in shared
-// memory, coalesced along the channels and once per element rather than once
-// per lane; then every warp scans the tile; then the threads finish their own
-// elements (skip, gate) and store them.  Sums and states are float32.
+// A CTA of 8 warps holds adjacent channels of one group and one sequence (32 of
+// them at N = 16).  Its threads first turn a tile of tokens into d, d x (and
+// dr) in shared memory, coalesced along the channels and once per element
+// rather than once per lane; then every warp scans the tile; then the threads
+// finish their own elements (skip, gate) and store them.  Sums and states are
+// float32.  (Four states a lane need a tenth fewer instructions but have half
+// the warps, and few rows are what this operator usually gets.)
 //
 // Bounds: one exp per state and token in the forward (16 a clock and SM: 3.6
 // ps per channel-token at N = 16 against 1.2 ps for its bytes) and two in the
-// backward, beside about 7 and 15 other float32 operations.
+// backward, beside the other float32 instructions of the step.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -74,8 +76,8 @@ __device__ __forceinline__ float exp2_unit(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float2 decay_of(float d, float2 rate) {
-    const float2 e = fma2(both(d), rate, both(3.f / 134217728.f));
+__device__ __forceinline__ float2 decay_of(float2 d, float2 rate) {
+    const float2 e = fma2(d, rate, both(3.f / 134217728.f));
     return make_float2(exp2_unit(e.x), exp2_unit(e.y));
 }
 
@@ -95,37 +97,44 @@ __device__ __forceinline__ float softplus_f(float x) {
 }
 
 template <int LPC> struct Geometry {
-    static constexpr int kStates = 4 * LPC;           // states a channel's lanes hold (N padded)
-    static constexpr int kChannels = kWarps * 32 / LPC;
+    static constexpr int kStates = 2 * LPC;           // states a channel's lanes hold (N padded)
     static constexpr int kPerWarp = 32 / LPC;         // channels per warp
-    static constexpr int kBatch = LPC < 4 ? 4 : LPC;  // tokens whose sums over the lanes are taken together
-    static constexpr int kTile = LPC <= 2 ? 8 * LPC : 32;                     // forward tile, tokens
+    static constexpr int kChannels = kWarps * kPerWarp;
+    static constexpr int kRows = kThreads / kChannels;  // token rows a pass of the CTA covers
+    static constexpr int kBatch = LPC < 8 ? 4 : 8;      // tokens whose sums over the lanes are taken together
+    static constexpr int kTile = LPC <= 2 ? 8 * LPC : 32;  // tokens of a tile
     static constexpr int kElems = kTile * kChannels / kThreads;
-    static constexpr int kRows = kThreads / kChannels;                        // token rows a pass of the CTA covers
     static constexpr int kPairs = (kTile * kStates + kThreads - 1) / kThreads;
     // row pitch of the sums: a batch's tokens fall into different banks
-    static constexpr int kPitch = LPC == 16 ? 34 : LPC == 1 ? 256 : LPC == 2 ? 136 : kChannels + kPerWarp;
+    static constexpr int kPitch = kChannels + (LPC >= 16 ? 4 : LPC == 1 ? 0 : LPC == 2 ? 8 : kPerWarp);
 };
 
-// Sums over a channel's LPC lanes of v[0 .. COUNT), each lane keeping COUNT /
-// LPC of them (all, when LPC is 1): lane `sub` ends with v[i] the sum of entry
-// sub * (COUNT / LPC) + i.  Halves are exchanged, so it takes COUNT - COUNT /
-// LPC shuffles rather than COUNT log2(LPC).
+// Sums over a channel's LPC lanes of v[0 .. COUNT): halves are exchanged, so
+// it takes about COUNT shuffles rather than COUNT log2(LPC).  Lane `sub` ends
+// with the sums of entries first_sum(sub) .. + kept_sums - 1 in v[0 ..).
 template <int COUNT, int LPC> __device__ __forceinline__ void lane_sums(float (&v)[COUNT], int sub) {
     int half = COUNT / 2;
 #pragma unroll
     for (int off = LPC / 2; off >= 1; off /= 2) {
-        const bool upper = (sub & off) != 0;
+        if (half > 0) {
+            const bool upper = (sub & off) != 0;
 #pragma unroll
-        for (int i = 0; i < COUNT / 2; ++i) {
-            if (i < half) {
-                const float send = upper ? v[i] : v[i + half];
-                const float keep = upper ? v[i + half] : v[i];
-                v[i] = keep + __shfl_xor_sync(0xffffffffu, send, off);
+            for (int i = 0; i < COUNT / 2; ++i) {
+                if (i < half) {
+                    const float send = upper ? v[i] : v[i + half];
+                    const float keep = upper ? v[i + half] : v[i];
+                    v[i] = keep + __shfl_xor_sync(0xffffffffu, send, off);
+                }
             }
+            half /= 2;
+        } else {
+            v[0] += __shfl_xor_sync(0xffffffffu, v[0], off);
         }
-        half /= 2;
     }
+}
+template <int COUNT, int LPC> __device__ constexpr int kept_sums() { return COUNT > LPC ? COUNT / LPC : 1; }
+template <int COUNT, int LPC> __device__ __forceinline__ int first_sum(int sub) {
+    return COUNT >= LPC ? sub * (COUNT / LPC) : sub / (LPC / COUNT);
 }
 
 struct Place {  // what a CTA works on
@@ -149,23 +158,20 @@ template <int LPC> __device__ __forceinline__ Place place_of(const ScanArgs &a, 
     return p;
 }
 
-// The four states n0 .. n0 + 3 of a lane in the order n0 + (j ^ m); those past N are zero.
-__device__ __forceinline__ void load_states(const float *p, int n0, int m, int states, float2 (&o)[2]) {
-    float v[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = p != nullptr && n0 + (j ^ m) < states ? p[j ^ m] : 0.f;
-    o[0] = make_float2(v[0], v[1]);
-    o[1] = make_float2(v[2], v[3]);
+// A lane's two states n0 + (0 ^ m), n0 + (1 ^ m); those past N are zero.
+__device__ __forceinline__ float2 load_states(const float *p, int n0, int m, int states) {
+    float2 v = both(0.f);
+    if (p != nullptr && n0 + m < states) v.x = p[m];
+    if (p != nullptr && n0 + (1 ^ m) < states) v.y = p[1 ^ m];
+    return v;
 }
-__device__ __forceinline__ void store_states(float *p, int n0, int m, int states, const float2 (&o)[2]) {
-    const float v[4] = {o[0].x, o[0].y, o[1].x, o[1].y};
-    if ((states & 3) == 0 && m == 0) {
-        if (n0 < states) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+__device__ __forceinline__ void store_states(float *p, int n0, int m, int states, float2 v) {
+    if ((states & 1) == 0) {
+        if (n0 < states) *reinterpret_cast<float2 *>(p) = m == 0 ? v : make_float2(v.y, v.x);
         return;
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (n0 + (j ^ m) < states) p[j ^ m] = v[j];
+    if (n0 + m < states) p[m] = v.x;
+    if (n0 + (1 ^ m) < states) p[1 ^ m] = v.y;
 }
 
 // Row of `saved` for token t (a multiple of kSegment) of a sequence: segments
@@ -174,44 +180,38 @@ __device__ __forceinline__ long segment_row(const Sequences &q, long s, long fir
     return (q.offsets == nullptr ? s * ((q.length + kSegment - 1) / kSegment) : first / kSegment + s) + t / kSegment;
 }
 
-// A tile's rows on their way from global to shared memory.
-template <typename T, int LPC> struct TileRows {
-    using G = Geometry<LPC>;
-    T x[G::kElems], s[G::kElems], z[G::kElems], k[G::kPairs], q[G::kPairs];
+// 1 / (1 + exp(-z)) of a gate.  Rows of 16 bits take the short form, whose
+// exponent is rounded first (|z| 2^-24 of the result, far below the rows' own
+// rounding).
+template <typename T> __device__ __forceinline__ float gate_sigmoid(float z) {
+    if (sizeof(T) == 4) return sigmoid_f(z);
+    return __fdividef(1.f, 1.f + __expf(-z));
+}
 
-    __device__ __forceinline__ void load(const ScanArgs &a, const Place &p, long t0, int ec, int er) {
-        const int count = static_cast<int>(min(static_cast<long>(G::kTile), p.end - t0));
-        const long row0 = p.first + t0;
-        const long cc = p.c0 + ec;
+// COUNT elements of a tile's rows, one channel, kRows tokens apart, from row
+// `p` on; those of tokens at or past `count` (all, when count is 0) are zero.
+template <typename T, int COUNT, int STEP>
+__device__ __forceinline__ void load_column(T (&o)[COUNT], const T *p, int stride, int t, int count) {
 #pragma unroll
-        for (int i = 0; i < G::kElems; ++i) {
-            const int t = er + i * G::kRows;
-            x[i] = s[i] = z[i] = from_float<T>(0.f);
-            if (ec < p.width && t < count) {
-                s[i] = static_cast<const T *>(a.steps)[(row0 + t) * a.step_stride + cc];
-                x[i] = static_cast<const T *>(a.values)[(row0 + t) * a.value_stride + cc];
-                if (a.gate != nullptr) z[i] = static_cast<const T *>(a.gate)[(row0 + t) * a.gate_stride + cc];
-            }
-        }
+    for (int i = 0; i < COUNT; ++i) o[i] = t + i * STEP < count ? p[i * STEP * stride] : from_float<T>(0.f);
+}
+
+// A tile's keys (or queries), N padded to kStates: entries threadIdx.x + i * kThreads.
+template <typename T, int COUNT, int STATES>
+__device__ __forceinline__ void load_keys(T (&o)[COUNT], const T *p, int stride, int states, int count) {
 #pragma unroll
-        for (int i = 0; i < G::kPairs; ++i) {
-            const int e = threadIdx.x + i * kThreads, t = e / G::kStates, n = e % G::kStates;
-            k[i] = q[i] = from_float<T>(0.f);
-            if (t < count && n < a.states) {
-                const long col = static_cast<long>(p.group) * a.states + n;
-                k[i] = static_cast<const T *>(a.keys)[(row0 + t) * a.key_stride + col];
-                q[i] = static_cast<const T *>(a.queries)[(row0 + t) * a.query_stride + col];
-            }
-        }
+    for (int i = 0; i < COUNT; ++i) {
+        const int e = threadIdx.x + i * kThreads, t = e / STATES, n = e % STATES;
+        o[i] = t < count && n < states ? p[t * stride + n] : from_float<T>(0.f);
     }
-};
+}
 
 // The next tile's rows are loaded while this one is scanned.
-template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, 2) scan_forward(const ScanArgs a) {
+template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, 3) scan_forward(const ScanArgs a) {
     using G = Geometry<LPC>;
-    __shared__ float2 in_s[G::kTile][G::kChannels];  // (d, d x)
+    __shared__ float4 in_s[G::kTile][G::kChannels];  // (d, d, d x, d x): pairs for the packed arithmetic
     __shared__ float sum_s[G::kTile * G::kPitch];
-    __shared__ __align__(16) float k_s[G::kTile][G::kStates], q_s[G::kTile][G::kStates];
+    __shared__ __align__(16) float k_s[G::kTile * G::kStates], q_s[G::kTile * G::kStates];
     const int chunk = static_cast<int>(blockIdx.y);
     const Place p = place_of<LPC>(a, chunk);
     if (chunk > 0 && p.begin >= p.end) return;  // past the end
@@ -222,70 +222,85 @@ template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, 2) sc
     const long cc = p.c0 + ec;
     const float bias = own && a.step_bias != nullptr ? a.step_bias[cc] : 0.f;
     const float skip = own && a.skip != nullptr ? a.skip[cc] : 0.f;
-    // scan: channel c, states n0 .. n0 + 3
-    const int sub = lane % LPC, c = tid / 32 * G::kPerWarp + lane / LPC, n0 = 4 * sub;
+    // scan: channel c, states n0 and n0 + 1
+    const int sub = lane % LPC, c = tid / 32 * G::kPerWarp + lane / LPC, n0 = 2 * sub;
     const bool live = c < p.width && n0 < a.states;
     const long row = static_cast<long>(a.channels) * a.states, at = static_cast<long>(p.c0 + c) * a.states + n0;
-    float2 rate[2], h[2];
-    load_states(live ? a.rates + at : nullptr, n0, 0, a.states, rate);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) rate[j] = mul2(rate[j], both(kLog2e));
+    const float2 rate = mul2(load_states(live ? a.rates + at : nullptr, n0, 0, a.states), both(kLog2e));
     const float *start = chunk > 0 ? a.carry + (p.s * a.chunks + chunk - 1) * row
                          : a.state0 != nullptr ? a.state0 + p.s * row : nullptr;
-    load_states(live && start != nullptr ? start + at : nullptr, n0, 0, a.states, h);
+    float2 h = load_states(live && start != nullptr ? start + at : nullptr, n0, 0, a.states);
 
-    TileRows<T, LPC> next;
-    next.load(a, p, p.begin, ec, er);
+    T next_x[G::kElems], next_s[G::kElems], next_z[G::kElems], next_k[G::kPairs], next_q[G::kPairs];
+    auto load = [&](long t0) {
+        const int count = static_cast<int>(min(static_cast<long>(G::kTile), p.end - t0));
+        const long r = p.first + t0;
+        const int mine = own ? count : 0;
+        load_column<T, G::kElems, G::kRows>(next_s, static_cast<const T *>(a.steps) + (r + er) * a.step_stride + cc,
+                                            static_cast<int>(a.step_stride), er, mine);
+        load_column<T, G::kElems, G::kRows>(next_x, static_cast<const T *>(a.values) + (r + er) * a.value_stride + cc,
+                                            static_cast<int>(a.value_stride), er, mine);
+        if (a.gate != nullptr)
+            load_column<T, G::kElems, G::kRows>(next_z, static_cast<const T *>(a.gate) + (r + er) * a.gate_stride + cc,
+                                                static_cast<int>(a.gate_stride), er, mine);
+        const long col = static_cast<long>(p.group) * a.states;
+        load_keys<T, G::kPairs, G::kStates>(next_k, static_cast<const T *>(a.keys) + r * a.key_stride + col,
+                                            static_cast<int>(a.key_stride), a.states, count);
+        load_keys<T, G::kPairs, G::kStates>(next_q, static_cast<const T *>(a.queries) + r * a.query_stride + col,
+                                            static_cast<int>(a.query_stride), a.states, count);
+    };
+    if (p.begin < p.end) load(p.begin);
     for (long t0 = p.begin; t0 < p.end; t0 += G::kTile) {
         const int count = static_cast<int>(min(static_cast<long>(G::kTile), p.end - t0));
         T x[G::kElems], z[G::kElems];
 #pragma unroll
         for (int i = 0; i < G::kElems; ++i) {
             const int t = er + i * G::kRows;
-            x[i] = next.x[i];
-            z[i] = next.z[i];
-            float d = to_float(next.s[i]) + bias;
+            x[i] = next_x[i];
+            z[i] = next_z[i];
+            float d = to_float(next_s[i]) + bias;
             if (a.softplus) d = softplus_f(d);
             if (!own || t >= count) d = 0.f;
-            in_s[t][ec] = make_float2(d, d * to_float(x[i]));
+            const float dx = d * to_float(x[i]);
+            in_s[t][ec] = make_float4(d, d, dx, dx);
         }
 #pragma unroll
         for (int i = 0; i < G::kPairs; ++i) {
             const int e = tid + i * kThreads;
             if (G::kTile * G::kStates % kThreads == 0 || e < G::kTile * G::kStates) {
-                (&k_s[0][0])[e] = to_float(next.k[i]);
-                (&q_s[0][0])[e] = to_float(next.q[i]);
+                k_s[e] = to_float(next_k[i]);
+                q_s[e] = to_float(next_q[i]);
             }
         }
         __syncthreads();
-        if (t0 + G::kTile < p.end) next.load(a, p, t0 + G::kTile, ec, er);
+        if (t0 + G::kTile < p.end) load(t0 + G::kTile);
         for (int tb = 0; tb < count; tb += G::kBatch) {
             if (a.saved != nullptr && (t0 + tb) % kSegment == 0 && live)
                 store_states(a.saved + segment_row(a.seq, p.s, p.first, t0 + tb) * row + at, n0, 0, a.states, h);
             float sum[G::kBatch];
 #pragma unroll
             for (int u = 0; u < G::kBatch; ++u) {
-                const float2 in = in_s[tb + u][c];
-                const float4 k = *reinterpret_cast<const float4 *>(&k_s[tb + u][n0]);
-                const float4 q = *reinterpret_cast<const float4 *>(&q_s[tb + u][n0]);
-                h[0] = fma2(decay_of(in.x, rate[0]), h[0], mul2(both(in.y), make_float2(k.x, k.y)));
-                h[1] = fma2(decay_of(in.x, rate[1]), h[1], mul2(both(in.y), make_float2(k.z, k.w)));
-                const float2 y = fma2(make_float2(q.z, q.w), h[1], mul2(make_float2(q.x, q.y), h[0]));
+                const float4 in = in_s[tb + u][c];
+                const float2 k = *reinterpret_cast<const float2 *>(&k_s[(tb + u) * G::kStates + n0]);
+                const float2 q = *reinterpret_cast<const float2 *>(&q_s[(tb + u) * G::kStates + n0]);
+                h = fma2(decay_of(make_float2(in.x, in.y), rate), h, mul2(make_float2(in.z, in.w), k));
+                const float2 y = mul2(q, h);
                 sum[u] = y.x + y.y;
             }
             lane_sums<G::kBatch, LPC>(sum, sub);
 #pragma unroll
-            for (int i = 0; i < G::kBatch / LPC; ++i)
-                sum_s[(tb + sub * (G::kBatch / LPC) + i) * G::kPitch + c] = sum[i];
+            for (int i = 0; i < kept_sums<G::kBatch, LPC>(); ++i)
+                sum_s[(tb + first_sum<G::kBatch, LPC>(sub) + i) * G::kPitch + c] = sum[i];
         }
         __syncthreads();
+        T *out = static_cast<T *>(a.out) + (p.first + t0 + er) * a.channels + cc;
 #pragma unroll
         for (int i = 0; i < G::kElems; ++i) {
             const int t = er + i * G::kRows;
             if (own && t < count) {
                 float y = fmaf(skip, to_float(x[i]), sum_s[t * G::kPitch + ec]);
-                if (a.gate != nullptr) y *= to_float(z[i]) * sigmoid_f(to_float(z[i]));
-                static_cast<T *>(a.out)[(p.first + t0 + t) * a.channels + cc] = from_float<T>(y);
+                if (a.gate != nullptr) y *= to_float(z[i]) * gate_sigmoid<T>(to_float(z[i]));
+                out[i * G::kRows * a.channels] = from_float<T>(y);
             }
         }
         // no barrier here: the next tile's in_s, k_s and q_s were last read before the one above, and its
@@ -299,10 +314,10 @@ template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, 2) sc
 // BACKWARD: the same of the adjoint, which enters at the chunk's end:
 // g -> exp(A D) g + local with g_{t-1} = a_t (q_t dr_t + g_t).
 template <typename T, int LPC, bool BACKWARD>
-__global__ void __launch_bounds__(kThreads, 3) scan_local(const ScanArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) scan_local(const ScanArgs a) {
     using G = Geometry<LPC>;
-    __shared__ float2 in_s[G::kTile][G::kChannels];  // (d, d x) or (d, dr)
-    __shared__ __align__(16) float k_s[G::kTile][G::kStates];
+    __shared__ float4 in_s[G::kTile][G::kChannels];  // (d, d, d x, d x) or (d, d, dr, dr)
+    __shared__ __align__(16) float k_s[G::kTile * G::kStates];
     const int chunk = static_cast<int>(blockIdx.y) + (BACKWARD ? 1 : 0);
     const Place p = place_of<LPC>(a, chunk);
     const int tid = threadIdx.x, lane = tid & 31;
@@ -310,16 +325,14 @@ __global__ void __launch_bounds__(kThreads, 3) scan_local(const ScanArgs a) {
     const bool own = ec < p.width;
     const long cc = p.c0 + ec;
     const float bias = own && a.step_bias != nullptr ? a.step_bias[cc] : 0.f;
-    const int sub = lane % LPC, c = tid / 32 * G::kPerWarp + lane / LPC, n0 = 4 * sub;
+    const int sub = lane % LPC, c = tid / 32 * G::kPerWarp + lane / LPC, n0 = 2 * sub;
     const bool live = c < p.width && n0 < a.states;
     const long row = static_cast<long>(a.channels) * a.states, at = static_cast<long>(p.c0 + c) * a.states + n0;
-    float2 rate[2], h[2] = {both(0.f), both(0.f)};
-    load_states(live ? a.rates + at : nullptr, n0, 0, a.states, rate);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) rate[j] = mul2(rate[j], both(kLog2e));
+    const float2 rate = mul2(load_states(live ? a.rates + at : nullptr, n0, 0, a.states), both(kLog2e));
+    float2 h = both(0.f);
     float span = 0.f;
 
-    const T *steps = static_cast<const T *>(a.steps), *gate = static_cast<const T *>(a.gate);
+    const T *gate = static_cast<const T *>(a.gate);
     const T *in = static_cast<const T *>(BACKWARD ? a.grad_out : a.values);
     const T *keys = static_cast<const T *>(BACKWARD ? a.queries : a.keys);
     const long in_stride = BACKWARD ? a.channels : a.value_stride;
@@ -329,23 +342,17 @@ __global__ void __launch_bounds__(kThreads, 3) scan_local(const ScanArgs a) {
     auto load = [&](long tile) {
         const long t0 = p.begin + (BACKWARD ? tiles - 1 - tile : tile) * G::kTile;
         const int count = static_cast<int>(min(static_cast<long>(G::kTile), p.end - t0));
-#pragma unroll
-        for (int i = 0; i < G::kElems; ++i) {
-            const int t = er + i * G::kRows;
-            x[i] = s[i] = z[i] = from_float<T>(0.f);
-            if (own && t < count) {
-                s[i] = steps[(p.first + t0 + t) * a.step_stride + cc];
-                if (in != nullptr) x[i] = in[(p.first + t0 + t) * in_stride + cc];
-                if (BACKWARD && gate != nullptr) z[i] = gate[(p.first + t0 + t) * a.gate_stride + cc];
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < G::kPairs; ++i) {
-            const int e = tid + i * kThreads, t = e / G::kStates, n = e % G::kStates;
-            k[i] = t < count && n < a.states
-                       ? keys[(p.first + t0 + t) * key_stride + static_cast<long>(p.group) * a.states + n]
-                       : from_float<T>(0.f);
-        }
+        const long r = p.first + t0;
+        const int mine = own ? count : 0;
+        load_column<T, G::kElems, G::kRows>(s, static_cast<const T *>(a.steps) + (r + er) * a.step_stride + cc,
+                                            static_cast<int>(a.step_stride), er, mine);
+        load_column<T, G::kElems, G::kRows>(x, in + (r + er) * in_stride + cc, static_cast<int>(in_stride), er,
+                                            in == nullptr ? 0 : mine);
+        if (BACKWARD && gate != nullptr)
+            load_column<T, G::kElems, G::kRows>(z, gate + (r + er) * a.gate_stride + cc,
+                                                static_cast<int>(a.gate_stride), er, mine);
+        load_keys<T, G::kPairs, G::kStates>(k, keys + r * key_stride + static_cast<long>(p.group) * a.states,
+                                            static_cast<int>(key_stride), a.states, count);
         return count;
     };
     int count = tiles > 0 ? load(0) : 0;
@@ -356,30 +363,25 @@ __global__ void __launch_bounds__(kThreads, 3) scan_local(const ScanArgs a) {
             float d = to_float(s[i]) + bias, v = to_float(x[i]);
             if (a.softplus) d = softplus_f(d);
             if (!own || t >= count) d = 0.f;
-            if (BACKWARD && gate != nullptr) v *= to_float(z[i]) * sigmoid_f(to_float(z[i]));
+            if (BACKWARD && gate != nullptr) v *= to_float(z[i]) * gate_sigmoid<T>(to_float(z[i]));
+            if (!BACKWARD) v *= d;
             span += d;
-            in_s[t][ec] = make_float2(d, BACKWARD ? v : d * v);
+            in_s[t][ec] = make_float4(d, d, v, v);
         }
 #pragma unroll
         for (int i = 0; i < G::kPairs; ++i) {
             const int e = tid + i * kThreads;
-            if (G::kTile * G::kStates % kThreads == 0 || e < G::kTile * G::kStates) (&k_s[0][0])[e] = to_float(k[i]);
+            if (G::kTile * G::kStates % kThreads == 0 || e < G::kTile * G::kStates) k_s[e] = to_float(k[i]);
         }
         __syncthreads();
         if (tile + 1 < tiles) count = load(tile + 1);
-#pragma unroll 4
+#pragma unroll 8
         for (int i = 0; i < G::kTile; ++i) {
             const int t = BACKWARD ? G::kTile - 1 - i : i;
-            const float2 v = in_s[t][c];
-            const float4 kk = *reinterpret_cast<const float4 *>(&k_s[t][n0]);
-            const float2 a0 = decay_of(v.x, rate[0]), a1 = decay_of(v.x, rate[1]);
-            if (BACKWARD) {
-                h[0] = mul2(a0, fma2(both(v.y), make_float2(kk.x, kk.y), h[0]));
-                h[1] = mul2(a1, fma2(both(v.y), make_float2(kk.z, kk.w), h[1]));
-            } else {
-                h[0] = fma2(a0, h[0], mul2(both(v.y), make_float2(kk.x, kk.y)));
-                h[1] = fma2(a1, h[1], mul2(both(v.y), make_float2(kk.z, kk.w)));
-            }
+            const float4 v = in_s[t][c];
+            const float2 kk = *reinterpret_cast<const float2 *>(&k_s[t * G::kStates + n0]);
+            const float2 e = decay_of(make_float2(v.x, v.y), rate), w = make_float2(v.z, v.w);
+            h = BACKWARD ? mul2(e, fma2(w, kk, h)) : fma2(e, h, mul2(w, kk));
         }
         __syncthreads();
     }
@@ -406,6 +408,7 @@ template <bool BACKWARD> __global__ void __launch_bounds__(kThreads) scan_join(c
     const float rate = a.rates[at] * kLog2e;
     const float *start = BACKWARD ? a.grad_state1 : a.state0;
     float h = start != nullptr ? start[i] : 0.f;
+#pragma unroll 4
     for (int k = 0; k + 1 < a.chunks; ++k) {
         const long entry = s * a.chunks + (BACKWARD ? a.chunks - 1 - k : k);
         h = fmaf(exp2f(a.span[entry * a.channels + c] * rate), h, a.carry[entry * row + at]);
@@ -415,11 +418,13 @@ template <bool BACKWARD> __global__ void __launch_bounds__(kThreads) scan_join(c
 
 template <int LPC> struct BackwardShared {
     using G = Geometry<LPC>;
-    static constexpr int kCopies = G::kPerWarp >= 4 ? 4 : 2;
-    float4 in[kSegment][G::kChannels];     // d, d x, dr, x
-    float2 slopes[kSegment][G::kChannels]; // d's slope in the step, dy silu'(z)
+    static constexpr int kCopies = G::kPerWarp >= 2 ? 2 : 1;
+    float4 in[kSegment][G::kChannels];      // d, d, d x, d x
+    float2 dr[kSegment][G::kChannels];      // dr, dr
+    float x[kSegment][G::kChannels];
+    float2 slopes[kSegment][G::kChannels];  // d's slope in the step, dy silu'(z)
     float gk[kSegment * G::kPitch], ga[kSegment * G::kPitch], r[kSegment * G::kPitch];
-    // keys and queries, once for every order n ^ m of a lane's four states
+    // keys and queries, in either order n ^ m of a lane's two states
     alignas(16) float k[kSegment][kCopies][G::kStates];
     alignas(16) float q[kSegment][kCopies][G::kStates];
     float part[kWarps][kSegment][2 * G::kStates];
@@ -427,21 +432,23 @@ template <int LPC> struct BackwardShared {
 
 // One CTA walks a chunk's segments of kSegment tokens from the last to the
 // first: each is replayed from the state the forward saved at its start, its 16
-// states kept in registers, then the adjoint runs back over them.  Keys' and
-// queries' gradients are summed over the warp's channels by exchanges, over the
-// CTA's warps in shared memory and written as one row per channel tile of
-// key_part [tiles][tokens][2][N]; rates', skip's and step bias's as one row per
-// chunk.  All are added up afterwards in a fixed order.
+// states kept in registers, then the adjoint runs back over them; the segment
+// before it is loaded meanwhile.  Keys' and queries' gradients are summed over
+// the warp's channels by exchanges, over the CTA's warps in shared memory and
+// written as one row per channel tile of key_part [tiles][tokens][2][N];
+// rates', skip's and step bias's as one row per chunk.  All are added up
+// afterwards in a fixed order.
 //
-// A lane holds its four states in the order j ^ m, m from two of the bits that
-// tell the warp's channels apart.  The two halves of an exchange over such a
-// bit then are the same registers in every lane, so summing four states over
-// four channels needs no selects (of 7 exchanges a token, 1 has them).
-template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, LPC < 2 ? 1 : 2)
+// A lane holds its two states in the order j ^ m, m the lowest bit that tells
+// the warp's channels apart.  The two halves of the exchange over that bit then
+// are the same registers in every lane and need no selects.
+template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, LPC < 4 ? 1 : 3)
 scan_backward(const ScanArgs a) {
     using G = Geometry<LPC>;
     using S = BackwardShared<LPC>;
-    constexpr int kElems = kSegment * G::kChannels / kThreads;
+    constexpr int kElems = (kSegment * G::kChannels + kThreads - 1) / kThreads;
+    constexpr int kPairs = (kSegment * G::kStates + kThreads - 1) / kThreads;
+    constexpr int kBatch = 4;
     extern __shared__ __align__(16) unsigned char raw[];
     S &sh = *reinterpret_cast<S *>(raw);
     const long tile = blockIdx.x % a.tiles;
@@ -453,168 +460,167 @@ scan_backward(const ScanArgs a) {
     const long cc = p.c0 + ec;
     const float bias = own && a.step_bias != nullptr ? a.step_bias[cc] : 0.f;
     const float skip = own && a.skip != nullptr ? a.skip[cc] : 0.f;
-    const int sub = lane % LPC, in_warp = lane / LPC, c = warp * G::kPerWarp + in_warp, n0 = 4 * sub;
-    const int m = (in_warp & 1) * 2 + (G::kPerWarp >= 4 ? (in_warp >> 1) & 1 : 0);
-    const int copy = G::kPerWarp >= 4 ? m : m / 2;
+    const int sub = lane % LPC, in_warp = lane / LPC, c = warp * G::kPerWarp + in_warp, n0 = 2 * sub;
+    const int m = in_warp & 1;
     const bool live = c < p.width && n0 < a.states;
     const long row = static_cast<long>(a.channels) * a.states, at = static_cast<long>(p.c0 + c) * a.states + n0;
-    float2 rate[2], g[2], grate[2] = {both(0.f), both(0.f)};
-    load_states(live ? a.rates + at : nullptr, n0, m, a.states, rate);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) rate[j] = mul2(rate[j], both(kLog2e));
+    const float2 rate = mul2(load_states(live ? a.rates + at : nullptr, n0, m, a.states), both(kLog2e));
+    float2 grate = both(0.f);
     const float *start = chunk < a.chunks - 1 ? a.carry + (p.s * a.chunks + chunk + 1) * row
                          : a.grad_state1 != nullptr ? a.grad_state1 + p.s * row : nullptr;
-    load_states(live && start != nullptr ? start + at : nullptr, n0, m, a.states, g);
+    float2 g = load_states(live && start != nullptr ? start + at : nullptr, n0, m, a.states);
     float gskip = 0.f, gbias = 0.f;
 
-    const T *values = static_cast<const T *>(a.values), *steps = static_cast<const T *>(a.steps);
-    const T *keys = static_cast<const T *>(a.keys), *queries = static_cast<const T *>(a.queries);
-    const T *gate = static_cast<const T *>(a.gate), *gy = static_cast<const T *>(a.grad_out);
+    T next_x[kElems], next_s[kElems], next_z[kElems], next_g[kElems], next_k[kPairs], next_q[kPairs];
+    float2 next_h;
+    auto load = [&](long t0) {
+        const int count = static_cast<int>(min(static_cast<long>(kSegment), p.end - t0));
+        const long r = p.first + t0;
+        const int mine = own ? count : 0;
+        load_column<T, kElems, G::kRows>(next_s, static_cast<const T *>(a.steps) + (r + er) * a.step_stride + cc,
+                                         static_cast<int>(a.step_stride), er, mine);
+        load_column<T, kElems, G::kRows>(next_x, static_cast<const T *>(a.values) + (r + er) * a.value_stride + cc,
+                                         static_cast<int>(a.value_stride), er, mine);
+        load_column<T, kElems, G::kRows>(next_g, static_cast<const T *>(a.grad_out) + (r + er) * a.channels + cc,
+                                         a.channels, er, a.grad_out == nullptr ? 0 : mine);
+        if (a.gate != nullptr)
+            load_column<T, kElems, G::kRows>(next_z, static_cast<const T *>(a.gate) + (r + er) * a.gate_stride + cc,
+                                             static_cast<int>(a.gate_stride), er, mine);
+        const long col = static_cast<long>(p.group) * a.states;
+        load_keys<T, kPairs, G::kStates>(next_k, static_cast<const T *>(a.keys) + r * a.key_stride + col,
+                                         static_cast<int>(a.key_stride), a.states, count);
+        load_keys<T, kPairs, G::kStates>(next_q, static_cast<const T *>(a.queries) + r * a.query_stride + col,
+                                         static_cast<int>(a.query_stride), a.states, count);
+        next_h = load_states(live ? a.saved + segment_row(a.seq, p.s, p.first, t0) * row + at : nullptr, n0, m,
+                             a.states);
+    };
     const long segments = (p.end - p.begin + kSegment - 1) / kSegment;
+    if (segments > 0) load(p.begin + (segments - 1) * kSegment);
     for (long seg = segments - 1; seg >= 0; --seg) {
         const long t0 = p.begin + seg * kSegment;
         const int count = static_cast<int>(min(static_cast<long>(kSegment), p.end - t0));
 #pragma unroll
         for (int i = 0; i < kElems; ++i) {
             const int t = er + i * G::kRows;
-            float x = 0.f, d = 0.f, slope = 0.f, dr = 0.f, gz = 0.f;
-            if (own && t < count) {
-                const long r = p.first + t0 + t;
-                d = to_float(steps[r * a.step_stride + cc]) + bias;
-                x = to_float(values[r * a.value_stride + cc]);
-                dr = gy == nullptr ? 0.f : to_float(gy[r * a.channels + cc]);
-                slope = 1.f;
-                if (a.softplus) {
-                    slope = sigmoid_f(d);
-                    d = softplus_f(d);
-                }
-                if (gate != nullptr) {
-                    const float z = to_float(gate[r * a.gate_stride + cc]), sg = sigmoid_f(z);
-                    gz = dr * sg * fmaf(z, 1.f - sg, 1.f);
-                    dr *= z * sg;
-                }
+            if (G::kRows > kSegment && t >= kSegment) break;  // more threads than elements
+            const float x = to_float(next_x[i]);
+            float d = to_float(next_s[i]) + bias, dr = to_float(next_g[i]), slope = 1.f, gz = 0.f;
+            if (a.softplus) {
+                slope = sigmoid_f(d);
+                d = softplus_f(d);
             }
-            sh.in[t][ec] = make_float4(d, d * x, dr, x);
-            sh.slopes[t][ec] = make_float2(slope, gz);  // read back by this thread only
+            if (!own || t >= count) d = 0.f;
+            if (a.gate != nullptr) {
+                const float z = to_float(next_z[i]), sg = gate_sigmoid<T>(z);
+                gz = dr * sg * fmaf(z, 1.f - sg, 1.f);
+                dr *= z * sg;
+            }
+            const float dx = d * x;
+            sh.in[t][ec] = make_float4(d, d, dx, dx);
+            sh.dr[t][ec] = both(dr);
+            sh.x[t][ec] = x;                        // this and the next are read back by this thread only
+            sh.slopes[t][ec] = make_float2(slope, gz);
         }
-        for (int i = tid; i < kSegment * G::kStates; i += kThreads) {
-            const int t = i / G::kStates, n = i % G::kStates;
-            const bool ok = t < count && n < a.states;
-            const long r = p.first + t0 + t, col = static_cast<long>(p.group) * a.states + n;
-            const float k = ok ? to_float(keys[r * a.key_stride + col]) : 0.f;
-            const float q = ok ? to_float(queries[r * a.query_stride + col]) : 0.f;
 #pragma unroll
-            for (int o = 0; o < S::kCopies; ++o) {
-                const int order = S::kCopies == 4 ? o : 2 * o;
-                sh.k[t][o][n ^ order] = k;
-                sh.q[t][o][n ^ order] = q;
+        for (int i = 0; i < kPairs; ++i) {
+            const int e = tid + i * kThreads, t = e / G::kStates, n = e % G::kStates;
+            if (kSegment * G::kStates % kThreads == 0 || e < kSegment * G::kStates) {
+#pragma unroll
+                for (int o = 0; o < S::kCopies; ++o) {
+                    sh.k[t][o][n ^ o] = to_float(next_k[i]);
+                    sh.q[t][o][n ^ o] = to_float(next_q[i]);
+                }
             }
         }
+        float2 h[kSegment + 1];  // h[t] before token t of the segment, h[t + 1] after it
+        h[0] = next_h;
         __syncthreads();
-        float2 h[kSegment + 1][2];  // h[t] before token t of the segment, h[t + 1] after it
-        load_states(live ? a.saved + segment_row(a.seq, p.s, p.first, t0) * row + at : nullptr, n0, m, a.states, h[0]);
+        if (seg > 0) load(t0 - kSegment);
 #pragma unroll
         for (int t = 0; t < kSegment; ++t) {
-            if (t % 4 == 0) asm volatile("" ::: "memory");  // as below
-            const float2 in = *reinterpret_cast<const float2 *>(&sh.in[t][c]);
-            const float4 k = *reinterpret_cast<const float4 *>(&sh.k[t][copy][n0]);
-            h[t + 1][0] = fma2(decay_of(in.x, rate[0]), h[t][0], mul2(both(in.y), make_float2(k.x, k.y)));
-            h[t + 1][1] = fma2(decay_of(in.x, rate[1]), h[t][1], mul2(both(in.y), make_float2(k.z, k.w)));
+            if (t % 8 == 0) asm volatile("" ::: "memory");  // as below
+            const float4 in = sh.in[t][c];
+            const float2 k = *reinterpret_cast<const float2 *>(&sh.k[t][S::kCopies == 2 ? m : 0][n0]);
+            h[t + 1] = fma2(decay_of(make_float2(in.x, in.y), rate), h[t], mul2(make_float2(in.z, in.w), k));
         }
 #pragma unroll
-        for (int tb = kSegment - G::kBatch; tb >= 0; tb -= G::kBatch) {
-            float sk[G::kBatch], sa[G::kBatch], sr[G::kBatch];
+        for (int tb = kSegment - kBatch; tb >= 0; tb -= kBatch) {
+            float sk[kBatch], sa[kBatch], sr[kBatch];
             asm volatile("" ::: "memory");  // keeps the compiler from loading later batches early, which spills
 #pragma unroll
-            for (int u = G::kBatch - 1; u >= 0; --u) {
+            for (int u = kBatch - 1; u >= 0; --u) {
                 const int t = tb + u;
                 const float4 in = sh.in[t][c];
-                const float4 k4 = *reinterpret_cast<const float4 *>(&sh.k[t][copy][n0]);
-                const float4 q4 = *reinterpret_cast<const float4 *>(&sh.q[t][copy][n0]);
-                const float2 k[2] = {make_float2(k4.x, k4.y), make_float2(k4.z, k4.w)};
-                const float2 q[2] = {make_float2(q4.x, q4.y), make_float2(q4.z, q4.w)};
-                float2 dq[2], dk[2], pk = both(0.f), pa = both(0.f), pr = both(0.f);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float2 gh = fma2(q[j], both(in.z), g[j]);
-                    dq[j] = mul2(both(in.z), h[t + 1][j]);
-                    dk[j] = mul2(gh, both(in.y));
-                    pr = fma2(q[j], h[t + 1][j], pr);
-                    pk = fma2(gh, k[j], pk);
-                    g[j] = mul2(decay_of(in.x, rate[j]), gh);
-                    const float2 moved = mul2(g[j], h[t][j]);
-                    pa = fma2(moved, rate[j], pa);
-                    grate[j] = fma2(moved, both(in.x), grate[j]);
-                }
+                const float2 d = make_float2(in.x, in.y), dx = make_float2(in.z, in.w), dr = sh.dr[t][c];
+                const float2 k = *reinterpret_cast<const float2 *>(&sh.k[t][S::kCopies == 2 ? m : 0][n0]);
+                const float2 q = *reinterpret_cast<const float2 *>(&sh.q[t][S::kCopies == 2 ? m : 0][n0]);
+                const float2 gh = fma2(q, dr, g), dq = mul2(dr, h[t + 1]), dk = mul2(gh, dx);
+                const float2 pr = mul2(q, h[t + 1]), pk = mul2(gh, k);
+                g = mul2(decay_of(d, rate), gh);
+                const float2 moved = mul2(g, h[t]), pa = mul2(moved, rate);
+                grate = fma2(moved, d, grate);
                 sk[u] = pk.x + pk.y;
                 sa[u] = pa.x + pa.y;
                 sr[u] = pr.x + pr.y;
-                // over the warp's channels: states j and j ^ 2, then j ^ 1, then queries and keys
-                float vq[2] = {dq[0].x + __shfl_xor_sync(0xffffffffu, dq[1].x, LPC),
-                               dq[0].y + __shfl_xor_sync(0xffffffffu, dq[1].y, LPC)};
-                float vk[2] = {dk[0].x + __shfl_xor_sync(0xffffffffu, dk[1].x, LPC),
-                               dk[0].y + __shfl_xor_sync(0xffffffffu, dk[1].y, LPC)};
+                // over the warp's channels: the states' exchange, then queries against keys, then plain sums
                 float *part = sh.part[warp][t] + n0;
-                if (G::kPerWarp == 2) {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        part[j ^ m] = vq[j];
-                        part[G::kStates + (j ^ m)] = vk[j];
-                    }
+                if (G::kPerWarp == 1) {
+                    *reinterpret_cast<float2 *>(part) = dq;
+                    *reinterpret_cast<float2 *>(part + G::kStates) = dk;
                 } else {
-                    vq[0] += __shfl_xor_sync(0xffffffffu, vq[1], 2 * LPC);
-                    vk[0] += __shfl_xor_sync(0xffffffffu, vk[1], 2 * LPC);
-                    if (G::kPerWarp == 4) {
-                        part[m] = vq[0];
-                        part[G::kStates + m] = vk[0];
+                    const float vq = dq.x + __shfl_xor_sync(0xffffffffu, dq.y, LPC);
+                    const float vk = dk.x + __shfl_xor_sync(0xffffffffu, dk.y, LPC);
+                    if (G::kPerWarp == 2) {
+                        part[m] = vq;
+                        part[G::kStates + m] = vk;
                     } else {
-                        const bool keys_here = (in_warp & 4) != 0;
-                        float v = (keys_here ? vk[0] : vq[0]) +
-                                  __shfl_xor_sync(0xffffffffu, keys_here ? vq[0] : vk[0], 4 * LPC);
+                        const bool keys_here = (in_warp & 2) != 0;
+                        float v = (keys_here ? vk : vq) +
+                                  __shfl_xor_sync(0xffffffffu, keys_here ? vq : vk, 2 * LPC);
 #pragma unroll
-                        for (int off = 8 * LPC; off < 32; off *= 2) v += __shfl_xor_sync(0xffffffffu, v, off);
+                        for (int off = 4 * LPC; off < 32; off *= 2) v += __shfl_xor_sync(0xffffffffu, v, off);
                         part[(keys_here ? G::kStates : 0) + m] = v;
                     }
                 }
             }
-            lane_sums<G::kBatch, LPC>(sk, sub);
-            lane_sums<G::kBatch, LPC>(sa, sub);
-            lane_sums<G::kBatch, LPC>(sr, sub);
+            lane_sums<kBatch, LPC>(sk, sub);
+            lane_sums<kBatch, LPC>(sa, sub);
+            lane_sums<kBatch, LPC>(sr, sub);
 #pragma unroll
-            for (int i = 0; i < G::kBatch / LPC; ++i) {
-                const int o = (tb + sub * (G::kBatch / LPC) + i) * G::kPitch + c;
+            for (int i = 0; i < kept_sums<kBatch, LPC>(); ++i) {
+                const int o = (tb + first_sum<kBatch, LPC>(sub) + i) * G::kPitch + c;
                 sh.gk[o] = sk[i];
                 sh.ga[o] = sa[i];
                 sh.r[o] = sr[i];
             }
         }
         __syncthreads();
+        const long at_row = (p.first + t0 + er) * a.channels + cc;
 #pragma unroll
         for (int i = 0; i < kElems; ++i) {
             const int t = er + i * G::kRows;
             if (own && t < count) {
-                const long r = p.first + t0 + t;
+                const long r = at_row + i * G::kRows * a.channels;
                 const int o = t * G::kPitch + ec;
-                const float4 in = sh.in[t][ec];
+                const float x = sh.x[t][ec], dr = sh.dr[t][ec].x;
                 const float2 slope = sh.slopes[t][ec];
-                const float gd = fmaf(in.w, sh.gk[o], kLn2 * sh.ga[o]) * slope.x;  // rates were in powers of two
-                static_cast<T *>(a.grad_values)[r * a.channels + cc] = from_float<T>(fmaf(in.x, sh.gk[o], skip * in.z));
-                static_cast<T *>(a.grad_steps)[r * a.channels + cc] = from_float<T>(gd);
-                if (gate != nullptr)
-                    static_cast<T *>(a.grad_gate)[r * a.channels + cc] =
-                        from_float<T>(slope.y * fmaf(skip, in.w, sh.r[o]));
+                const float gd = fmaf(x, sh.gk[o], kLn2 * sh.ga[o]) * slope.x;  // rates were in powers of two
+                static_cast<T *>(a.grad_values)[r] = from_float<T>(fmaf(sh.in[t][ec].x, sh.gk[o], skip * dr));
+                static_cast<T *>(a.grad_steps)[r] = from_float<T>(gd);
+                if (a.gate != nullptr)
+                    static_cast<T *>(a.grad_gate)[r] = from_float<T>(slope.y * fmaf(skip, x, sh.r[o]));
                 gbias += gd;
-                gskip = fmaf(in.z, in.w, gskip);
+                gskip = fmaf(dr, x, gskip);
             }
         }
+        float *key_part = a.key_part + (tile * a.seq.tokens + p.first + t0) * 2 * a.states;
         for (int i = tid; i < count * 2 * G::kStates; i += kThreads) {
             const int t = i / (2 * G::kStates), e = i % (2 * G::kStates);
             float v = 0.f;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) v += sh.part[w][t][e];
             const int which = e / G::kStates, n = e % G::kStates;
-            if (n < a.states)
-                a.key_part[((tile * a.seq.tokens + p.first + t0 + t) * 2 + which) * a.states + n] = v;
+            if (n < a.states) key_part[(t * 2 + which) * a.states + n] = v;
         }
         __syncthreads();
     }
@@ -623,7 +629,7 @@ scan_backward(const ScanArgs a) {
         store_states(a.grad_state0 + p.s * row + at, n0, m, a.states, g);
     if (live) store_states(a.rate_part + entry * row + at, n0, m, a.states, grate);
     // the skip's and step bias's sums over the CTA's token rows
-    float *cs = sh.gk;  // [2][kRows][kChannels]
+    float *cs = reinterpret_cast<float *>(&sh.in[0][0]);  // [2][kRows][kChannels]
     cs[er * G::kChannels + ec] = gskip;
     cs[(G::kRows + er) * G::kChannels + ec] = gbias;
     __syncthreads();
@@ -673,40 +679,30 @@ __global__ void __launch_bounds__(kThreads) scan_sum_rows(const ScanArgs a, floa
     *out = v;
 }
 
-template <typename T> __device__ __forceinline__ void load_row(const T *p, int n0, int states, float2 (&o)[2]) {
-    float v[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = n0 + j < states ? to_float(p[j]) : 0.f;
-    o[0] = make_float2(v[0], v[1]);
-    o[1] = make_float2(v[2], v[3]);
-}
-
 // One token per sequence, the states [sequences][channels][N] moved on in place.
 template <typename T, int LPC> __global__ void __launch_bounds__(kThreads) scan_step(const ScanArgs a, float *state) {
     const long id = static_cast<long>(blockIdx.x) * kThreads + threadIdx.x;
     const long row = id / LPC;  // sequence * channels + channel
-    const int sub = static_cast<int>(id % LPC), n0 = 4 * sub;
+    const int sub = static_cast<int>(id % LPC), n0 = 2 * sub;
     const bool ok = row < a.seq.count * a.channels;
-    const bool live = ok && n0 < a.states;
+    const bool live = ok && n0 < a.states, second = n0 + 1 < a.states;
     const long s = ok ? row / a.channels : 0, c = ok ? row % a.channels : 0;
-    const long group = c / a.group_channels, col = group * a.states + n0;
+    const long col = c / a.group_channels * a.states + n0;
     float sum = 0.f, x = 0.f;
     if (live) {
         x = to_float(static_cast<const T *>(a.values)[s * a.value_stride + c]);
         float d = to_float(static_cast<const T *>(a.steps)[s * a.step_stride + c]);
         if (a.step_bias != nullptr) d += a.step_bias[c];
-        float2 h[2], rate[2], k[2], q[2];
-        load_states(state + row * a.states + n0, n0, 0, a.states, h);
-        load_states(a.rates + c * a.states + n0, n0, 0, a.states, rate);
-        load_row(static_cast<const T *>(a.keys) + s * a.key_stride + col, n0, a.states, k);
-        load_row(static_cast<const T *>(a.queries) + s * a.query_stride + col, n0, a.states, q);
+        float2 h = load_states(state + row * a.states + n0, n0, 0, a.states);
+        const float2 rate = load_states(a.rates + c * a.states + n0, n0, 0, a.states);
+        const T *k = static_cast<const T *>(a.keys) + s * a.key_stride + col;
+        const T *q = static_cast<const T *>(a.queries) + s * a.query_stride + col;
+        const float2 kk = make_float2(to_float(k[0]), second ? to_float(k[1]) : 0.f);
+        const float2 qq = make_float2(to_float(q[0]), second ? to_float(q[1]) : 0.f);
         if (a.softplus) d = softplus_f(d);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            h[j] = fma2(decay_of(d, mul2(rate[j], both(kLog2e))), h[j], mul2(both(d * x), k[j]));
-            const float2 y = mul2(q[j], h[j]);
-            sum += y.x + y.y;
-        }
+        h = fma2(decay_of(both(d), mul2(rate, both(kLog2e))), h, mul2(both(d * x), kk));
+        const float2 y = mul2(qq, h);
+        sum = y.x + y.y;
         store_states(state + row * a.states + n0, n0, 0, a.states, h);
     }
 #pragma unroll
@@ -715,7 +711,7 @@ template <typename T, int LPC> __global__ void __launch_bounds__(kThreads) scan_
         if (a.skip != nullptr) sum = fmaf(a.skip[c], x, sum);
         if (a.gate != nullptr) {
             const float z = to_float(static_cast<const T *>(a.gate)[s * a.gate_stride + c]);
-            sum *= z * sigmoid_f(z);
+            sum *= z * gate_sigmoid<T>(z);
         }
         static_cast<T *>(a.out)[s * a.channels + c] = from_float<T>(sum);
     }
@@ -723,7 +719,7 @@ template <typename T, int LPC> __global__ void __launch_bounds__(kThreads) scan_
 
 int lanes_per_channel(int states) {
     int lpc = 1;
-    while (4 * lpc < states) lpc *= 2;
+    while (2 * lpc < states) lpc *= 2;
     return lpc;
 }
 
@@ -820,7 +816,8 @@ template <typename T> int launch_lanes(ScanKind kind, const ScanArgs &a, cudaStr
         case 2: return launch_kind<T, 2>(kind, a, st);
         case 4: return launch_kind<T, 4>(kind, a, st);
         case 8: return launch_kind<T, 8>(kind, a, st);
-        default: return launch_kind<T, 16>(kind, a, st);
+        case 16: return launch_kind<T, 16>(kind, a, st);
+        default: return launch_kind<T, 32>(kind, a, st);
     }
 }
 int launch_scan(ScanKind kind, int dtype, const ScanArgs &a, cudaStream_t st) {
@@ -842,6 +839,14 @@ int check_scan(const char *what, int dtype, int channels, int states, int groups
         return fail(BSSM_ERR_INVALID, "%s: rows do not divide into sequences of one length", what);
     if (sequences > 0x7fffffffL / channels) return fail(BSSM_ERR_INVALID, "%s: too many rows", what);  // the grid
     return BSSM_OK;
+}
+
+// A tile's rows are addressed by 32-bit offsets from its first one.
+bool strides_fit(const ScanArgs &a) {
+    for (long stride : {a.value_stride, a.step_stride, a.key_stride, a.query_stride, a.gate_stride,
+                        static_cast<long>(a.channels)})
+        if (stride < 0 || stride > 0x7fffffffL / 64) return false;
+    return true;
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -888,6 +893,7 @@ extern "C" int bssm_selective_scan(const void *values, long value_stride, const 
     a.seq.offsets = offsets;
     a.softplus = softplus;
     a.out = out; a.state1 = state1; a.saved = saved;
+    if (!strides_fit(a)) return fail(BSSM_ERR_UNSUPPORTED, "selective_scan: row stride too large");
     set_forward_chunks(a, longest);
     const long needed = place_carry(a, workspace);
     if (workspace_floats < needed || (needed > 0 && workspace == nullptr))
@@ -933,6 +939,7 @@ extern "C" int bssm_selective_scan_backward(
     a.softplus = softplus;
     a.saved = const_cast<float *>(saved); a.grad_out = grad_out; a.grad_state1 = grad_state1;
     a.grad_values = grad_values; a.grad_steps = grad_steps; a.grad_gate = grad_gate; a.grad_state0 = grad_state0;
+    if (!strides_fit(a)) return fail(BSSM_ERR_UNSUPPORTED, "selective_scan_backward: row stride too large");
     set_backward_chunks(a, longest);
     const long needed = place_backward(a, workspace);
     if (workspace_floats < needed || (needed > 0 && workspace == nullptr))
