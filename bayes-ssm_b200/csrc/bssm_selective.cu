@@ -14,8 +14,8 @@
 //   dd   = sum_n g (A a h_{t-1} + x k),  dA = sum_t g d a h_{t-1},  a = exp(d A)
 //
 // Work split.  A lane holds 2 states of a channel and LPC = ceil(N / 2) lanes
-// (a power of two, 1..32) hold the channel, so the sums over N take log2(LPC)
-// exchanges and a warp advances 32 / LPC channels; tokens are walked in order.
+// (a power of two, 1..32) hold the channel, so a warp advances 32 / LPC
+// channels; tokens are walked in order.
 // A CTA of 8 warps holds adjacent channels of one group and one sequence (32 of
 // them at N = 16).  Its threads first turn a tile of tokens into d, d x (and
 // dr) in shared memory, coalesced along the channels and once per element
@@ -30,6 +30,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "bayes_ssm_b200.h"
 #include "bssm_internal.h"
@@ -76,23 +77,33 @@ __device__ __forceinline__ float exp2_unit(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float2 decay_of(float2 d, float2 rate) {
-    const float2 e = fma2(d, rate, both(3.f / 134217728.f));
+__device__ __forceinline__ float2 decay_of(float d, float2 rate) {
+    const float2 e = fma2(both(d), rate, both(3.f / 134217728.f));
     return make_float2(exp2_unit(e.x), exp2_unit(e.y));
 }
 
-// log(1 + exp(x)) = max(x, 0) + log1p(exp(-|x|)), and log1p(e) = 2 atanh(e / (2 + e)) = 2 v P(v^2) with
+// log(1 + exp(x)) = max(x, 0) + log1p(e) with e = exp(-|x|), and log1p(e) = 2 atanh(v) = 2 v P(v^2) with
 // v = e / (2 + e) in (0, 1/3]; P is atanh(v) / v fitted for the least relative error over v^2 in (0, 1/9], 2^-27.9
-// (iterated weighted least squares).  A step's error is one of the decay's exponent, so expf, which keeps the bits
-// that rounding x log2 e would lose.
-__device__ __forceinline__ float softplus_f(float x) {
-    const float e = expf(-fabsf(x));
-    const float v = __fdividef(e, 2.f + e), w = v * v;
+// (iterated weighted least squares).  A step's error is one of the decay's exponent, so e is taken with what
+// rounding |x| log2 e lost: 2^(t + l) = 2^t (1 + l ln 2).  The slope is e's too: 1 / (1 + e) or e / (1 + e).
+__device__ __forceinline__ float reciprocal(float x) {  // within 1 ulp
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <bool SLOPE> __device__ __forceinline__ float softplus_f(float x, float &slope) {
+    constexpr float kLog2eLow = 1.925963033500e-8f;  // log2 e beyond its first 24 bits
+    const float y = fabsf(x) > 128.f ? -128.f : -fabsf(x);  // a NaN stays one
+    const float t = y * kLog2e, l = fmaf(y, kLog2eLow, fmaf(y, kLog2e, -t));
+    float e = exp2_unit(t);
+    e = fmaf(e, l * kLn2, e);
+    const float v = e * reciprocal(2.f + e), w = v * v;
     float p = 0.14089173f;
     p = fmaf(p, w, 0.13980305f);
     p = fmaf(p, w, 0.20012454f);
     p = fmaf(p, w, 0.33333157f);
     p = fmaf(p, w, 1.f);
+    if (SLOPE) slope = (x >= 0.f ? 1.f : e) * reciprocal(1.f + e);
     return fmaf(2.f * v, p, fmaxf(x, 0.f));
 }
 
@@ -101,40 +112,42 @@ template <int LPC> struct Geometry {
     static constexpr int kPerWarp = 32 / LPC;         // channels per warp
     static constexpr int kChannels = kWarps * kPerWarp;
     static constexpr int kRows = kThreads / kChannels;  // token rows a pass of the CTA covers
-    static constexpr int kBatch = LPC < 8 ? 4 : 8;      // tokens whose sums over the lanes are taken together
     static constexpr int kTile = LPC <= 2 ? 8 * LPC : 32;  // tokens of a tile
     static constexpr int kElems = kTile * kChannels / kThreads;
-    static constexpr int kPairs = (kTile * kStates + kThreads - 1) / kThreads;
-    // row pitch of the sums: a batch's tokens fall into different banks
-    static constexpr int kPitch = kChannels + (LPC >= 16 ? 4 : LPC == 1 ? 0 : LPC == 2 ? 8 : kPerWarp);
+    static constexpr int kPairs = (kTile * LPC + kThreads - 1) / kThreads;  // pairs of states a thread loads
 };
 
-// Sums over a channel's LPC lanes of v[0 .. COUNT): halves are exchanged, so
-// it takes about COUNT shuffles rather than COUNT log2(LPC).  Lane `sub` ends
-// with the sums of entries first_sum(sub) .. + kept_sums - 1 in v[0 ..).
-template <int COUNT, int LPC> __device__ __forceinline__ void lane_sums(float (&v)[COUNT], int sub) {
-    int half = COUNT / 2;
-#pragma unroll
-    for (int off = LPC / 2; off >= 1; off /= 2) {
-        if (half > 0) {
-            const bool upper = (sub & off) != 0;
-#pragma unroll
-            for (int i = 0; i < COUNT / 2; ++i) {
-                if (i < half) {
-                    const float send = upper ? v[i] : v[i + half];
-                    const float keep = upper ? v[i + half] : v[i];
-                    v[i] = keep + __shfl_xor_sync(0xffffffffu, send, off);
-                }
-            }
-            half /= 2;
-        } else {
-            v[0] += __shfl_xor_sync(0xffffffffu, v[0], off);
-        }
+// Sums over a channel's lanes go through shared memory: every lane leaves its
+// term at [token][thread], and the thread that finishes the element adds the
+// LPC neighbours (a store per token and a few wide loads per element; exchanges
+// between the lanes would take a shuffle, an add and two selects a token).  The
+// 16-byte loads of 8 neighbouring elements start at different vectors, so that
+// they fall into different banks.
+template <int LPC> __device__ __forceinline__ float sum_of(const float *token, int c) {
+    if (LPC == 1) return token[c];
+    if (LPC == 2) {
+        const float2 v = reinterpret_cast<const float2 *>(token)[c];
+        return v.x + v.y;
     }
+    constexpr int kVecs = LPC < 4 ? 1 : LPC / 4, kShift = LPC == 8 ? 2 : LPC == 16 ? 1 : 0;
+    float2 sum = both(0.f);
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) {
+        const float4 v = reinterpret_cast<const float4 *>(token)[c * kVecs + ((j + (c >> kShift)) & (kVecs - 1))];
+        sum = __fadd2_rn(sum, __fadd2_rn(make_float2(v.x, v.y), make_float2(v.z, v.w)));
+    }
+    return sum.x + sum.y;
 }
-template <int COUNT, int LPC> __device__ constexpr int kept_sums() { return COUNT > LPC ? COUNT / LPC : 1; }
-template <int COUNT, int LPC> __device__ __forceinline__ int first_sum(int sub) {
-    return COUNT >= LPC ? sub * (COUNT / LPC) : sub / (LPC / COUNT);
+template <int LPC> __device__ __forceinline__ float2 sums_of(const float2 *token, int c) {
+    if (LPC == 1) return token[c];
+    constexpr int kVecs = LPC < 2 ? 1 : LPC / 2, kShift = LPC == 4 ? 2 : LPC == 8 ? 1 : 0;
+    float2 sum = both(0.f);
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) {
+        const float4 v = reinterpret_cast<const float4 *>(token)[c * kVecs + ((j + (c >> kShift)) & (kVecs - 1))];
+        sum = __fadd2_rn(sum, __fadd2_rn(make_float2(v.x, v.y), make_float2(v.z, v.w)));
+    }
+    return sum;
 }
 
 struct Place {  // what a CTA works on
@@ -151,8 +164,9 @@ template <int LPC> __device__ __forceinline__ Place place_of(const ScanArgs &a, 
     const int in_group = (tile - p.group * a.tiles_per_group) * Geometry<LPC>::kChannels;
     p.c0 = p.group * a.group_channels + in_group;
     p.width = min(Geometry<LPC>::kChannels, a.group_channels - in_group);
-    p.first = a.seq.begin(p.s);
-    p.tokens = max(0L, a.seq.end(p.s) - p.first);
+    // the same in every lane: said to the compiler, which then keeps addresses in uniform registers
+    p.first = __shfl_sync(0xffffffffu, a.seq.begin(p.s), 0);
+    p.tokens = __shfl_sync(0xffffffffu, max(0L, a.seq.end(p.s) - p.first), 0);
     p.begin = min(p.tokens, chunk * a.chunk);
     p.end = chunk == a.chunks - 1 ? p.tokens : min(p.tokens, p.begin + a.chunk);
     return p;
@@ -185,33 +199,91 @@ __device__ __forceinline__ long segment_row(const Sequences &q, long s, long fir
 // rounding).
 template <typename T> __device__ __forceinline__ float gate_sigmoid(float z) {
     if (sizeof(T) == 4) return sigmoid_f(z);
-    return __fdividef(1.f, 1.f + __expf(-z));
+    return reciprocal(1.f + exp2_unit(-kLog2e * z));
 }
 
-// COUNT elements of a tile's rows, one channel, kRows tokens apart, from row
-// `p` on; those of tokens at or past `count` (all, when count is 0) are zero.
-template <typename T, int COUNT, int STEP>
-__device__ __forceinline__ void load_column(T (&o)[COUNT], const T *p, int stride, int t, int count) {
+// An element between its load and its use: a whole register each.  As 16-bit
+// variables, two of them are packed into one right behind their loads, which
+// then wait there instead of running on under the tile before.
+template <typename T> struct Raw {
+    unsigned bits;
+    __device__ __forceinline__ void load(const T *p) { bits = *reinterpret_cast<const unsigned short *>(p); }
+    __device__ __forceinline__ float value() const;
+};
+template <> __device__ __forceinline__ float Raw<__nv_bfloat16>::value() const { return __uint_as_float(bits << 16); }
+template <> __device__ __forceinline__ float Raw<__half>::value() const {
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+}
+template <> struct Raw<float> {
+    unsigned bits;
+    __device__ __forceinline__ void load(const float *p) { bits = __float_as_uint(*p); }
+    __device__ __forceinline__ float value() const { return __uint_as_float(bits); }
+};
+
+// The rows of one operand as a CTA's threads read (or write) them, a tile of
+// tokens at a time: the tile's first row and the CTA's first channel are the
+// same for all threads (64 bits, moved on tile by tile), and what a thread adds
+// to them is small.
+template <typename T> struct Rows {
+    T *tile;                // the tile's first row, at the CTA's first channel
+    long advance;           // from one tile to the next
+    unsigned offset, step;  // a thread's first element, and from one of its elements to the next
+    __device__ __forceinline__ Rows(const void *p, long stride, long row, long c0, int t, int c, int rows, int tokens)
+        : tile(const_cast<T *>(static_cast<const T *>(p)) + row * stride + c0), advance(tokens * stride),
+          offset(t * static_cast<unsigned>(stride) + c), step(rows * static_cast<unsigned>(stride)) {}
+    // o[i] is the element i * ROWS tokens on, zero where there is none; WHOLE: all of them exist
+    template <bool WHOLE, int COUNT, int ROWS>
+    __device__ __forceinline__ void load(Raw<T> (&o)[COUNT], int t, int count) {
 #pragma unroll
-    for (int i = 0; i < COUNT; ++i) o[i] = t + i * STEP < count ? p[i * STEP * stride] : from_float<T>(0.f);
-}
+        for (int i = 0; i < COUNT; ++i) {
+            if (!WHOLE) o[i].bits = 0;
+            if (WHOLE || t + i * ROWS < count) o[i].load(tile + (offset + i * step));
+        }
+        tile += advance;
+    }
+    __device__ __forceinline__ void store(int i, float v) const { tile[offset + i * step] = from_float<T>(v); }
+};
 
-// A tile's keys (or queries), N padded to kStates: entries threadIdx.x + i * kThreads.
+// A tile's keys or queries, N padded to STATES, two states at a time: entries
+// threadIdx.x + i * kThreads of [tile][STATES / 2].  PAIRED: both in one load
+// (16-bit types: both in `first`).
+template <typename T> struct KeyPair {
+    Raw<T> first, second;
+    __device__ __forceinline__ float2 value(bool paired) const {
+        if (sizeof(T) == 4 || !paired) return make_float2(first.value(), second.value());
+        return make_float2(Raw<T>{first.bits & 0xffffu}.value(), Raw<T>{first.bits >> 16}.value());
+    }
+};
 template <typename T, int COUNT, int STATES>
-__device__ __forceinline__ void load_keys(T (&o)[COUNT], const T *p, int stride, int states, int count) {
+__device__ __forceinline__ void load_keys(KeyPair<T> (&o)[COUNT], const T *&p, unsigned stride, long advance,
+                                          int states, int count, bool paired) {
 #pragma unroll
     for (int i = 0; i < COUNT; ++i) {
-        const int e = threadIdx.x + i * kThreads, t = e / STATES, n = e % STATES;
-        o[i] = t < count && n < states ? p[t * stride + n] : from_float<T>(0.f);
+        const unsigned e = threadIdx.x + i * kThreads, t = e / (STATES / 2), n = e % (STATES / 2) * 2;
+        o[i].first.bits = o[i].second.bits = 0;
+        if (t >= static_cast<unsigned>(count) || n >= static_cast<unsigned>(states)) continue;
+        const T *q = p + (t * stride + n);
+        if (sizeof(T) == 2 && paired) {
+            o[i].first.bits = *reinterpret_cast<const unsigned *>(q);
+        } else {
+            o[i].first.load(q);
+            if (n + 1 < static_cast<unsigned>(states)) o[i].second.load(q + 1);
+        }
     }
+    p += advance;
+}
+template <typename T> __device__ __forceinline__ bool keys_paired(const void *p, long stride, int states) {
+    return (states & 1) == 0 && (stride & 1) == 0 && reinterpret_cast<uintptr_t>(p) % (2 * sizeof(T)) == 0;
 }
 
 // The next tile's rows are loaded while this one is scanned.
 template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, 3) scan_forward(const ScanArgs a) {
     using G = Geometry<LPC>;
-    __shared__ float4 in_s[G::kTile][G::kChannels];  // (d, d, d x, d x): pairs for the packed arithmetic
-    __shared__ float sum_s[G::kTile * G::kPitch];
-    __shared__ __align__(16) float k_s[G::kTile * G::kStates], q_s[G::kTile * G::kStates];
+    __shared__ float2 in_s[G::kTile][G::kChannels];  // (d, d x)
+    __shared__ float4 kq_s[G::kTile][LPC];           // (k, k, q, q) of a lane's states
+    // q . h of a lane's states, [kTile][kThreads]: an object of its own, so that loads of the two above may be moved
+    // over its stores
+    extern __shared__ __align__(16) float part_s[];
     const int chunk = static_cast<int>(blockIdx.y);
     const Place p = place_of<LPC>(a, chunk);
     if (chunk > 0 && p.begin >= p.end) return;  // past the end
@@ -231,80 +303,105 @@ template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, 3) sc
                          : a.state0 != nullptr ? a.state0 + p.s * row : nullptr;
     float2 h = load_states(live && start != nullptr ? start + at : nullptr, n0, 0, a.states);
 
-    T next_x[G::kElems], next_s[G::kElems], next_z[G::kElems], next_k[G::kPairs], next_q[G::kPairs];
-    auto load = [&](long t0) {
-        const int count = static_cast<int>(min(static_cast<long>(G::kTile), p.end - t0));
-        const long r = p.first + t0;
-        const int mine = own ? count : 0;
-        load_column<T, G::kElems, G::kRows>(next_s, static_cast<const T *>(a.steps) + (r + er) * a.step_stride + cc,
-                                            static_cast<int>(a.step_stride), er, mine);
-        load_column<T, G::kElems, G::kRows>(next_x, static_cast<const T *>(a.values) + (r + er) * a.value_stride + cc,
-                                            static_cast<int>(a.value_stride), er, mine);
-        if (a.gate != nullptr)
-            load_column<T, G::kElems, G::kRows>(next_z, static_cast<const T *>(a.gate) + (r + er) * a.gate_stride + cc,
-                                                static_cast<int>(a.gate_stride), er, mine);
-        const long col = static_cast<long>(p.group) * a.states;
-        load_keys<T, G::kPairs, G::kStates>(next_k, static_cast<const T *>(a.keys) + r * a.key_stride + col,
-                                            static_cast<int>(a.key_stride), a.states, count);
-        load_keys<T, G::kPairs, G::kStates>(next_q, static_cast<const T *>(a.queries) + r * a.query_stride + col,
-                                            static_cast<int>(a.query_stride), a.states, count);
+    const long row0 = p.first + p.begin;
+    Rows<T> values(a.values, a.value_stride, row0, p.c0, er, ec, G::kRows, G::kTile);
+    Rows<T> steps(a.steps, a.step_stride, row0, p.c0, er, ec, G::kRows, G::kTile);
+    Rows<T> gate(a.gate, a.gate_stride, row0, p.c0, er, ec, G::kRows, G::kTile);
+    Rows<T> out(a.out, a.channels, row0, p.c0, er, ec, G::kRows, G::kTile);
+    const T *keys = static_cast<const T *>(a.keys) + row0 * a.key_stride + static_cast<long>(p.group) * a.states;
+    const T *queries = static_cast<const T *>(a.queries) + row0 * a.query_stride + static_cast<long>(p.group) * a.states;
+    const long keys_on = G::kTile * a.key_stride, queries_on = G::kTile * a.query_stride;
+    const bool paired_k = keys_paired<T>(a.keys, a.key_stride, a.states);
+    const bool paired_q = keys_paired<T>(a.queries, a.query_stride, a.states);
+    float *saved = a.saved == nullptr ? nullptr : a.saved + segment_row(a.seq, p.s, p.first, p.begin) * row + at;
+    const bool full_width = p.width == G::kChannels;
+    Raw<T> next_x[G::kElems], next_s[G::kElems], next_z[G::kElems];
+    KeyPair<T> next_k[G::kPairs], next_q[G::kPairs];
+    auto load_rows = [&](auto whole, int count) {
+        constexpr bool kWhole = decltype(whole)::value;
+        steps.template load<kWhole, G::kElems, G::kRows>(next_s, er, count);
+        values.template load<kWhole, G::kElems, G::kRows>(next_x, er, count);
+        if (a.gate != nullptr) gate.template load<kWhole, G::kElems, G::kRows>(next_z, er, count);
     };
-    if (p.begin < p.end) load(p.begin);
-    for (long t0 = p.begin; t0 < p.end; t0 += G::kTile) {
-        const int count = static_cast<int>(min(static_cast<long>(G::kTile), p.end - t0));
-        T x[G::kElems], z[G::kElems];
+    auto load = [&](long left) {  // tokens from the tile's first on
+        const int count = static_cast<int>(min(static_cast<long>(G::kTile), left));
+        if (count == G::kTile && full_width) load_rows(std::true_type{}, count);
+        else load_rows(std::false_type{}, own ? count : 0);
+        load_keys<T, G::kPairs, G::kStates>(next_k, keys, static_cast<unsigned>(a.key_stride), keys_on, a.states, count,
+                                            paired_k);
+        load_keys<T, G::kPairs, G::kStates>(next_q, queries, static_cast<unsigned>(a.query_stride), queries_on,
+                                            a.states, count, paired_q);
+    };
+    long left = p.end - p.begin;
+    if (left > 0) load(left);
+    int phase = 0;  // the tile's first token in its segment
+    for (; left > 0; left -= G::kTile) {
+        const int count = static_cast<int>(min(static_cast<long>(G::kTile), left));
+        const bool whole = count == G::kTile && full_width;
+        Raw<T> x[G::kElems], z[G::kElems];
+        float d[G::kElems], unused;
 #pragma unroll
         for (int i = 0; i < G::kElems; ++i) {
-            const int t = er + i * G::kRows;
             x[i] = next_x[i];
             z[i] = next_z[i];
-            float d = to_float(next_s[i]) + bias;
-            if (a.softplus) d = softplus_f(d);
-            if (!own || t >= count) d = 0.f;
-            const float dx = d * to_float(x[i]);
-            in_s[t][ec] = make_float4(d, d, dx, dx);
+            d[i] = next_s[i].value() + bias;
+        }
+        if (a.softplus) {
+#pragma unroll
+            for (int i = 0; i < G::kElems; ++i) d[i] = softplus_f<false>(d[i], unused);
+        }
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < G::kElems; ++i)
+                if (!own || er + i * G::kRows >= count) d[i] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < G::kElems; ++i) {
+            in_s[er + i * G::kRows][ec] = make_float2(d[i], d[i] * x[i].value());
         }
 #pragma unroll
         for (int i = 0; i < G::kPairs; ++i) {
             const int e = tid + i * kThreads;
-            if (G::kTile * G::kStates % kThreads == 0 || e < G::kTile * G::kStates) {
-                k_s[e] = to_float(next_k[i]);
-                q_s[e] = to_float(next_q[i]);
+            if (G::kTile * LPC % kThreads == 0 || e < G::kTile * LPC) {
+                const float2 k = next_k[i].value(paired_k), q = next_q[i].value(paired_q);
+                (&kq_s[0][0])[e] = make_float4(k.x, k.y, q.x, q.y);
             }
         }
+        if (left > G::kTile) load(left - G::kTile);
         __syncthreads();
-        if (t0 + G::kTile < p.end) load(t0 + G::kTile);
-        for (int tb = 0; tb < count; tb += G::kBatch) {
-            if (a.saved != nullptr && (t0 + tb) % kSegment == 0 && live)
-                store_states(a.saved + segment_row(a.seq, p.s, p.first, t0 + tb) * row + at, n0, 0, a.states, h);
-            float sum[G::kBatch];
+        for (int tb = 0; tb < count; tb += 8) {
+            if (saved != nullptr && (phase + tb) % kSegment == 0) {
+                if (live) store_states(saved, n0, 0, a.states, h);
+                saved += row;
+            }
+            // what does not depend on h first: only one FMA a token does
+            float2 decay[8], inflow[8];
 #pragma unroll
-            for (int u = 0; u < G::kBatch; ++u) {
-                const float4 in = in_s[tb + u][c];
-                const float2 k = *reinterpret_cast<const float2 *>(&k_s[(tb + u) * G::kStates + n0]);
-                const float2 q = *reinterpret_cast<const float2 *>(&q_s[(tb + u) * G::kStates + n0]);
-                h = fma2(decay_of(make_float2(in.x, in.y), rate), h, mul2(make_float2(in.z, in.w), k));
+            for (int u = 0; u < 8; ++u) {
+                const float2 in = in_s[tb + u][c], k = *reinterpret_cast<const float2 *>(&kq_s[tb + u][sub]);
+                decay[u] = decay_of(in.x, rate);
+                inflow[u] = mul2(both(in.y), k);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float2 q = *(reinterpret_cast<const float2 *>(&kq_s[tb + u][sub]) + 1);
+                h = fma2(decay[u], h, inflow[u]);
                 const float2 y = mul2(q, h);
-                sum[u] = y.x + y.y;
+                part_s[(tb + u) * kThreads + tid] = y.x + y.y;
             }
-            lane_sums<G::kBatch, LPC>(sum, sub);
-#pragma unroll
-            for (int i = 0; i < kept_sums<G::kBatch, LPC>(); ++i)
-                sum_s[(tb + first_sum<G::kBatch, LPC>(sub) + i) * G::kPitch + c] = sum[i];
         }
         __syncthreads();
-        T *out = static_cast<T *>(a.out) + (p.first + t0 + er) * a.channels + cc;
 #pragma unroll
         for (int i = 0; i < G::kElems; ++i) {
             const int t = er + i * G::kRows;
-            if (own && t < count) {
-                float y = fmaf(skip, to_float(x[i]), sum_s[t * G::kPitch + ec]);
-                if (a.gate != nullptr) y *= to_float(z[i]) * gate_sigmoid<T>(to_float(z[i]));
-                out[i * G::kRows * a.channels] = from_float<T>(y);
-            }
+            float y = fmaf(skip, x[i].value(), sum_of<LPC>(part_s + t * kThreads, ec));
+            if (a.gate != nullptr) y *= z[i].value() * gate_sigmoid<T>(z[i].value());
+            if (whole || (own && t < count)) out.store(i, y);
         }
-        // no barrier here: the next tile's in_s, k_s and q_s were last read before the one above, and its
-        // sum_s is written after the next one
+        out.tile += out.advance;
+        phase = (phase + G::kTile) % kSegment;
+        // no barrier here: the next tile's in and kq were last read before the one above, and its part is written
+        // after the next one
     }
     if (live && a.state1 != nullptr && p.end == p.tokens) store_states(a.state1 + p.s * row + at, n0, 0, a.states, h);
 }
@@ -316,7 +413,7 @@ template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, 3) sc
 template <typename T, int LPC, bool BACKWARD>
 __global__ void __launch_bounds__(kThreads, 4) scan_local(const ScanArgs a) {
     using G = Geometry<LPC>;
-    __shared__ float4 in_s[G::kTile][G::kChannels];  // (d, d, d x, d x) or (d, d, dr, dr)
+    __shared__ float2 in_s[G::kTile][G::kChannels];  // (d, d x) or (d, dr)
     __shared__ __align__(16) float k_s[G::kTile * G::kStates];
     const int chunk = static_cast<int>(blockIdx.y) + (BACKWARD ? 1 : 0);
     const Place p = place_of<LPC>(a, chunk);
@@ -332,56 +429,79 @@ __global__ void __launch_bounds__(kThreads, 4) scan_local(const ScanArgs a) {
     float2 h = both(0.f);
     float span = 0.f;
 
-    const T *gate = static_cast<const T *>(a.gate);
-    const T *in = static_cast<const T *>(BACKWARD ? a.grad_out : a.values);
-    const T *keys = static_cast<const T *>(BACKWARD ? a.queries : a.keys);
-    const long in_stride = BACKWARD ? a.channels : a.value_stride;
-    const long key_stride = BACKWARD ? a.query_stride : a.key_stride;
     const long tiles = (p.end - p.begin + G::kTile - 1) / G::kTile;
-    T x[G::kElems], s[G::kElems], z[G::kElems], k[G::kPairs];
+    // BACKWARD walks the tiles from the last one down
+    const long row0 = p.first + p.begin + (BACKWARD && tiles > 0 ? (tiles - 1) * G::kTile : 0);
+    constexpr int kOn = BACKWARD ? -G::kTile : G::kTile;
+    Rows<T> in(BACKWARD ? a.grad_out : a.values, BACKWARD ? a.channels : a.value_stride, row0, p.c0, er, ec, G::kRows,
+               kOn);
+    Rows<T> steps(a.steps, a.step_stride, row0, p.c0, er, ec, G::kRows, kOn);
+    Rows<T> gate(a.gate, a.gate_stride, row0, p.c0, er, ec, G::kRows, kOn);
+    const bool gated = BACKWARD && a.gate != nullptr, present = !BACKWARD || a.grad_out != nullptr;
+    const long key_stride = BACKWARD ? a.query_stride : a.key_stride, keys_on = kOn * key_stride;
+    const void *all_keys = BACKWARD ? a.queries : a.keys;
+    const T *keys = static_cast<const T *>(all_keys) + row0 * key_stride + static_cast<long>(p.group) * a.states;
+    const bool paired = keys_paired<T>(all_keys, key_stride, a.states), full_width = p.width == G::kChannels;
+    Raw<T> x[G::kElems], s[G::kElems], z[G::kElems];
+    KeyPair<T> k[G::kPairs];
+    auto load_rows = [&](auto whole, int count) {
+        constexpr bool kWhole = decltype(whole)::value;
+        steps.template load<kWhole, G::kElems, G::kRows>(s, er, count);
+        if (present) in.template load<kWhole, G::kElems, G::kRows>(x, er, count);
+        else in.template load<false, G::kElems, G::kRows>(x, er, 0);
+        if (gated) gate.template load<kWhole, G::kElems, G::kRows>(z, er, count);
+    };
     auto load = [&](long tile) {
         const long t0 = p.begin + (BACKWARD ? tiles - 1 - tile : tile) * G::kTile;
         const int count = static_cast<int>(min(static_cast<long>(G::kTile), p.end - t0));
-        const long r = p.first + t0;
-        const int mine = own ? count : 0;
-        load_column<T, G::kElems, G::kRows>(s, static_cast<const T *>(a.steps) + (r + er) * a.step_stride + cc,
-                                            static_cast<int>(a.step_stride), er, mine);
-        load_column<T, G::kElems, G::kRows>(x, in + (r + er) * in_stride + cc, static_cast<int>(in_stride), er,
-                                            in == nullptr ? 0 : mine);
-        if (BACKWARD && gate != nullptr)
-            load_column<T, G::kElems, G::kRows>(z, gate + (r + er) * a.gate_stride + cc,
-                                                static_cast<int>(a.gate_stride), er, mine);
-        load_keys<T, G::kPairs, G::kStates>(k, keys + r * key_stride + static_cast<long>(p.group) * a.states,
-                                            static_cast<int>(key_stride), a.states, count);
+        if (count == G::kTile && full_width) load_rows(std::true_type{}, count);
+        else load_rows(std::false_type{}, own ? count : 0);
+        load_keys<T, G::kPairs, G::kStates>(k, keys, static_cast<unsigned>(key_stride), keys_on, a.states, count, paired);
         return count;
     };
     int count = tiles > 0 ? load(0) : 0;
     for (long tile = 0; tile < tiles; ++tile) {
+        const bool whole = count == G::kTile && full_width;
+        float d[G::kElems], unused;
+#pragma unroll
+        for (int i = 0; i < G::kElems; ++i) d[i] = s[i].value() + bias;
+        if (a.softplus) {
+#pragma unroll
+            for (int i = 0; i < G::kElems; ++i) d[i] = softplus_f<false>(d[i], unused);
+        }
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < G::kElems; ++i)
+                if (!own || er + i * G::kRows >= count) d[i] = 0.f;
+        }
 #pragma unroll
         for (int i = 0; i < G::kElems; ++i) {
-            const int t = er + i * G::kRows;
-            float d = to_float(s[i]) + bias, v = to_float(x[i]);
-            if (a.softplus) d = softplus_f(d);
-            if (!own || t >= count) d = 0.f;
-            if (BACKWARD && gate != nullptr) v *= to_float(z[i]) * gate_sigmoid<T>(to_float(z[i]));
-            if (!BACKWARD) v *= d;
-            span += d;
-            in_s[t][ec] = make_float4(d, d, v, v);
+            float v = x[i].value();
+            if (gated) v *= z[i].value() * gate_sigmoid<T>(z[i].value());
+            if (!BACKWARD) v *= d[i];
+            span += d[i];
+            in_s[er + i * G::kRows][ec] = make_float2(d[i], v);
         }
 #pragma unroll
         for (int i = 0; i < G::kPairs; ++i) {
             const int e = tid + i * kThreads;
-            if (G::kTile * G::kStates % kThreads == 0 || e < G::kTile * G::kStates) k_s[e] = to_float(k[i]);
+            if (G::kTile * LPC % kThreads == 0 || e < G::kTile * LPC)
+                reinterpret_cast<float2 *>(k_s)[e] = k[i].value(paired);
         }
-        __syncthreads();
         if (tile + 1 < tiles) count = load(tile + 1);
-#pragma unroll 8
-        for (int i = 0; i < G::kTile; ++i) {
-            const int t = BACKWARD ? G::kTile - 1 - i : i;
-            const float4 v = in_s[t][c];
-            const float2 kk = *reinterpret_cast<const float2 *>(&k_s[t * G::kStates + n0]);
-            const float2 e = decay_of(make_float2(v.x, v.y), rate), w = make_float2(v.z, v.w);
-            h = BACKWARD ? mul2(e, fma2(w, kk, h)) : fma2(e, h, mul2(w, kk));
+        __syncthreads();
+        for (int tb = 0; tb < G::kTile; tb += 8) {
+            float2 decay[8], inflow[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int t = BACKWARD ? G::kTile - 1 - (tb + u) : tb + u;
+                const float2 v = in_s[t][c], kk = *reinterpret_cast<const float2 *>(&k_s[t * G::kStates + n0]);
+                decay[u] = decay_of(v.x, rate);
+                inflow[u] = mul2(both(v.y), kk);
+                if (BACKWARD) inflow[u] = mul2(decay[u], inflow[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) h = fma2(decay[u], h, inflow[u]);
         }
         __syncthreads();
     }
@@ -419,14 +539,11 @@ template <bool BACKWARD> __global__ void __launch_bounds__(kThreads) scan_join(c
 template <int LPC> struct BackwardShared {
     using G = Geometry<LPC>;
     static constexpr int kCopies = G::kPerWarp >= 2 ? 2 : 1;
-    float4 in[kSegment][G::kChannels];      // d, d, d x, d x
-    float2 dr[kSegment][G::kChannels];      // dr, dr
-    float x[kSegment][G::kChannels];
+    float4 in[kSegment][G::kChannels];      // d, d x, dr, x
     float2 slopes[kSegment][G::kChannels];  // d's slope in the step, dy silu'(z)
-    float gk[kSegment * G::kPitch], ga[kSegment * G::kPitch], r[kSegment * G::kPitch];
-    // keys and queries, in either order n ^ m of a lane's two states
-    alignas(16) float k[kSegment][kCopies][G::kStates];
-    alignas(16) float q[kSegment][kCopies][G::kStates];
+    float4 kq[kSegment][kCopies][LPC];      // (k, k, q, q) of a lane's states, in either order j ^ m
+    float2 lane_ka[kSegment][kThreads];     // g . k and g . (A a h) of a lane's states
+    float lane_r[kSegment][kThreads];       // q . h
     float part[kWarps][kSegment][2 * G::kStates];
 };
 
@@ -442,13 +559,13 @@ template <int LPC> struct BackwardShared {
 // A lane holds its two states in the order j ^ m, m the lowest bit that tells
 // the warp's channels apart.  The two halves of the exchange over that bit then
 // are the same registers in every lane and need no selects.
-template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, LPC < 4 ? 1 : 3)
+template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, LPC < 4 ? 1 : 2)
 scan_backward(const ScanArgs a) {
     using G = Geometry<LPC>;
     using S = BackwardShared<LPC>;
     constexpr int kElems = (kSegment * G::kChannels + kThreads - 1) / kThreads;
-    constexpr int kPairs = (kSegment * G::kStates + kThreads - 1) / kThreads;
-    constexpr int kBatch = 4;
+    constexpr int kPairs = (kSegment * LPC + kThreads - 1) / kThreads;
+    constexpr int kBatch = 4;  // tokens between which loads are kept apart
     extern __shared__ __align__(16) unsigned char raw[];
     S &sh = *reinterpret_cast<S *>(raw);
     const long tile = blockIdx.x % a.tiles;
@@ -461,7 +578,9 @@ scan_backward(const ScanArgs a) {
     const float bias = own && a.step_bias != nullptr ? a.step_bias[cc] : 0.f;
     const float skip = own && a.skip != nullptr ? a.skip[cc] : 0.f;
     const int sub = lane % LPC, in_warp = lane / LPC, c = warp * G::kPerWarp + in_warp, n0 = 2 * sub;
-    const int m = in_warp & 1;
+    const int m = G::kPerWarp >= 2 ? in_warp & 1 : 0, copy = S::kCopies == 2 ? m : 0;
+    const bool keys_here = (in_warp & 2) != 0;
+    const int part_at = (keys_here ? G::kStates : 0) + n0 + m;
     const bool live = c < p.width && n0 < a.states;
     const long row = static_cast<long>(a.channels) * a.states, at = static_cast<long>(p.c0 + c) * a.states + n0;
     const float2 rate = mul2(load_states(live ? a.rates + at : nullptr, n0, m, a.states), both(kLog2e));
@@ -471,157 +590,193 @@ scan_backward(const ScanArgs a) {
     float2 g = load_states(live && start != nullptr ? start + at : nullptr, n0, m, a.states);
     float gskip = 0.f, gbias = 0.f;
 
-    T next_x[kElems], next_s[kElems], next_z[kElems], next_g[kElems], next_k[kPairs], next_q[kPairs];
-    float2 next_h;
-    auto load = [&](long t0) {
-        const int count = static_cast<int>(min(static_cast<long>(kSegment), p.end - t0));
-        const long r = p.first + t0;
-        const int mine = own ? count : 0;
-        load_column<T, kElems, G::kRows>(next_s, static_cast<const T *>(a.steps) + (r + er) * a.step_stride + cc,
-                                         static_cast<int>(a.step_stride), er, mine);
-        load_column<T, kElems, G::kRows>(next_x, static_cast<const T *>(a.values) + (r + er) * a.value_stride + cc,
-                                         static_cast<int>(a.value_stride), er, mine);
-        load_column<T, kElems, G::kRows>(next_g, static_cast<const T *>(a.grad_out) + (r + er) * a.channels + cc,
-                                         a.channels, er, a.grad_out == nullptr ? 0 : mine);
-        if (a.gate != nullptr)
-            load_column<T, kElems, G::kRows>(next_z, static_cast<const T *>(a.gate) + (r + er) * a.gate_stride + cc,
-                                             static_cast<int>(a.gate_stride), er, mine);
-        const long col = static_cast<long>(p.group) * a.states;
-        load_keys<T, kPairs, G::kStates>(next_k, static_cast<const T *>(a.keys) + r * a.key_stride + col,
-                                         static_cast<int>(a.key_stride), a.states, count);
-        load_keys<T, kPairs, G::kStates>(next_q, static_cast<const T *>(a.queries) + r * a.query_stride + col,
-                                         static_cast<int>(a.query_stride), a.states, count);
-        next_h = load_states(live ? a.saved + segment_row(a.seq, p.s, p.first, t0) * row + at : nullptr, n0, m,
-                             a.states);
-    };
     const long segments = (p.end - p.begin + kSegment - 1) / kSegment;
-    if (segments > 0) load(p.begin + (segments - 1) * kSegment);
-    for (long seg = segments - 1; seg >= 0; --seg) {
-        const long t0 = p.begin + seg * kSegment;
-        const int count = static_cast<int>(min(static_cast<long>(kSegment), p.end - t0));
+    const long row0 = p.first + p.begin + (segments > 0 ? (segments - 1) * kSegment : 0);  // walked from the last down
+    Rows<T> values(a.values, a.value_stride, row0, p.c0, er, ec, G::kRows, -kSegment);
+    Rows<T> steps(a.steps, a.step_stride, row0, p.c0, er, ec, G::kRows, -kSegment);
+    Rows<T> gate(a.gate, a.gate_stride, row0, p.c0, er, ec, G::kRows, -kSegment);
+    Rows<T> above(a.grad_out, a.channels, row0, p.c0, er, ec, G::kRows, -kSegment);
+    Rows<T> to_values(a.grad_values, a.channels, row0, p.c0, er, ec, G::kRows, -kSegment);
+    T *to_steps = static_cast<T *>(a.grad_steps) + row0 * a.channels + p.c0;
+    T *to_gate = static_cast<T *>(a.grad_gate) + row0 * a.channels + p.c0;
+    float *key_part = a.key_part + (tile * a.seq.tokens + row0) * 2 * a.states;
+    const T *keys = static_cast<const T *>(a.keys) + row0 * a.key_stride + static_cast<long>(p.group) * a.states;
+    const T *queries = static_cast<const T *>(a.queries) + row0 * a.query_stride + static_cast<long>(p.group) * a.states;
+    const bool paired_k = keys_paired<T>(a.keys, a.key_stride, a.states);
+    const bool paired_q = keys_paired<T>(a.queries, a.query_stride, a.states);
+    const bool full_width = p.width == G::kChannels && G::kRows <= kSegment;
+    Raw<T> next_x[kElems], next_s[kElems], next_z[kElems], next_g[kElems];
+    KeyPair<T> next_k[kPairs], next_q[kPairs];
+    float2 next_h;
+    auto load_rows = [&](auto whole, int count) {
+        constexpr bool kWhole = decltype(whole)::value;
+        steps.template load<kWhole, kElems, G::kRows>(next_s, er, count);
+        values.template load<kWhole, kElems, G::kRows>(next_x, er, count);
+        if (a.grad_out != nullptr) above.template load<kWhole, kElems, G::kRows>(next_g, er, count);
+        else above.template load<false, kElems, G::kRows>(next_g, er, 0);
+        if (a.gate != nullptr) gate.template load<kWhole, kElems, G::kRows>(next_z, er, count);
+    };
+    const float *saved = a.saved + segment_row(a.seq, p.s, p.first, row0 - p.first) * row + at;
+    auto load = [&](int count) {
+        if (count == kSegment && full_width) load_rows(std::true_type{}, count);
+        else load_rows(std::false_type{}, own ? count : 0);
+        load_keys<T, kPairs, G::kStates>(next_k, keys, static_cast<unsigned>(a.key_stride), -kSegment * a.key_stride,
+                                         a.states, count, paired_k);
+        load_keys<T, kPairs, G::kStates>(next_q, queries, static_cast<unsigned>(a.query_stride),
+                                         -kSegment * a.query_stride, a.states, count, paired_q);
+        next_h = load_states(live ? saved : nullptr, n0, m, a.states);
+        saved -= row;
+    };
+    // only the last segment may be short
+    int count = static_cast<int>(p.end - p.begin - (segments - 1) * kSegment);
+    if (segments > 0) load(count);
+    for (long seg = segments - 1; seg >= 0; --seg, count = kSegment) {
+        const bool whole = count == kSegment && full_width;
 #pragma unroll
         for (int i = 0; i < kElems; ++i) {
             const int t = er + i * G::kRows;
             if (G::kRows > kSegment && t >= kSegment) break;  // more threads than elements
-            const float x = to_float(next_x[i]);
-            float d = to_float(next_s[i]) + bias, dr = to_float(next_g[i]), slope = 1.f, gz = 0.f;
-            if (a.softplus) {
-                slope = sigmoid_f(d);
-                d = softplus_f(d);
-            }
-            if (!own || t >= count) d = 0.f;
+            const float x = next_x[i].value();
+            float d = next_s[i].value() + bias, dr = next_g[i].value(), slope = 1.f, gz = 0.f;
+            if (a.softplus) d = softplus_f<true>(d, slope);
+            if (!whole && (!own || t >= count)) d = 0.f;
             if (a.gate != nullptr) {
-                const float z = to_float(next_z[i]), sg = gate_sigmoid<T>(z);
+                const float z = next_z[i].value(), sg = gate_sigmoid<T>(z);
                 gz = dr * sg * fmaf(z, 1.f - sg, 1.f);
                 dr *= z * sg;
             }
             const float dx = d * x;
-            sh.in[t][ec] = make_float4(d, d, dx, dx);
-            sh.dr[t][ec] = both(dr);
-            sh.x[t][ec] = x;                        // this and the next are read back by this thread only
-            sh.slopes[t][ec] = make_float2(slope, gz);
+            sh.in[t][ec] = make_float4(d, dx, dr, x);
+            sh.slopes[t][ec] = make_float2(slope, gz);  // read back by this thread only
         }
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
-            const int e = tid + i * kThreads, t = e / G::kStates, n = e % G::kStates;
-            if (kSegment * G::kStates % kThreads == 0 || e < kSegment * G::kStates) {
-#pragma unroll
-                for (int o = 0; o < S::kCopies; ++o) {
-                    sh.k[t][o][n ^ o] = to_float(next_k[i]);
-                    sh.q[t][o][n ^ o] = to_float(next_q[i]);
-                }
+            const int e = tid + i * kThreads, t = e / LPC, n = e % LPC;
+            if (kSegment * LPC % kThreads == 0 || e < kSegment * LPC) {
+                const float2 k = next_k[i].value(paired_k), q = next_q[i].value(paired_q);
+                sh.kq[t][0][n] = make_float4(k.x, k.y, q.x, q.y);
+                if (S::kCopies == 2) sh.kq[t][S::kCopies - 1][n] = make_float4(k.y, k.x, q.y, q.x);
             }
         }
         float2 h[kSegment + 1];  // h[t] before token t of the segment, h[t + 1] after it
         h[0] = next_h;
+        if (seg > 0) load(kSegment);
         __syncthreads();
-        if (seg > 0) load(t0 - kSegment);
 #pragma unroll
-        for (int t = 0; t < kSegment; ++t) {
-            if (t % 8 == 0) asm volatile("" ::: "memory");  // as below
-            const float4 in = sh.in[t][c];
-            const float2 k = *reinterpret_cast<const float2 *>(&sh.k[t][S::kCopies == 2 ? m : 0][n0]);
-            h[t + 1] = fma2(decay_of(make_float2(in.x, in.y), rate), h[t], mul2(make_float2(in.z, in.w), k));
+        for (int tb = 0; tb < kSegment; tb += 8) {
+            asm volatile("" ::: "memory");  // as below
+            float2 decay[8], inflow[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float2 in = *reinterpret_cast<const float2 *>(&sh.in[tb + u][c]);
+                const float2 k = *reinterpret_cast<const float2 *>(&sh.kq[tb + u][copy][sub]);
+                decay[u] = decay_of(in.x, rate);
+                inflow[u] = mul2(both(in.y), k);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) h[tb + u + 1] = fma2(decay[u], h[tb + u], inflow[u]);
         }
 #pragma unroll
         for (int tb = kSegment - kBatch; tb >= 0; tb -= kBatch) {
-            float sk[kBatch], sa[kBatch], sr[kBatch];
             asm volatile("" ::: "memory");  // keeps the compiler from loading later batches early, which spills
+            float4 in[kBatch], kq[kBatch];
+            float2 decay[kBatch], out_ka[kBatch], vqk[kBatch];
+            float out_r[kBatch];
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                in[u] = sh.in[tb + u][c];
+                kq[u] = sh.kq[tb + u][copy][sub];
+            }
+            // what does not depend on the adjoint first
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                decay[u] = decay_of(in[u].x, rate);
+                const float2 pr = mul2(make_float2(kq[u].z, kq[u].w), h[tb + u + 1]);
+                out_r[u] = pr.x + pr.y;
+            }
+            float2 dk[kBatch];
 #pragma unroll
             for (int u = kBatch - 1; u >= 0; --u) {
-                const int t = tb + u;
-                const float4 in = sh.in[t][c];
-                const float2 d = make_float2(in.x, in.y), dx = make_float2(in.z, in.w), dr = sh.dr[t][c];
-                const float2 k = *reinterpret_cast<const float2 *>(&sh.k[t][S::kCopies == 2 ? m : 0][n0]);
-                const float2 q = *reinterpret_cast<const float2 *>(&sh.q[t][S::kCopies == 2 ? m : 0][n0]);
-                const float2 gh = fma2(q, dr, g), dq = mul2(dr, h[t + 1]), dk = mul2(gh, dx);
-                const float2 pr = mul2(q, h[t + 1]), pk = mul2(gh, k);
-                g = mul2(decay_of(d, rate), gh);
-                const float2 moved = mul2(g, h[t]), pa = mul2(moved, rate);
-                grate = fma2(moved, d, grate);
-                sk[u] = pk.x + pk.y;
-                sa[u] = pa.x + pa.y;
-                sr[u] = pr.x + pr.y;
-                // over the warp's channels: the states' exchange, then queries against keys, then plain sums
-                float *part = sh.part[warp][t] + n0;
-                if (G::kPerWarp == 1) {
-                    *reinterpret_cast<float2 *>(part) = dq;
-                    *reinterpret_cast<float2 *>(part + G::kStates) = dk;
-                } else {
-                    const float vq = dq.x + __shfl_xor_sync(0xffffffffu, dq.y, LPC);
-                    const float vk = dk.x + __shfl_xor_sync(0xffffffffu, dk.y, LPC);
-                    if (G::kPerWarp == 2) {
-                        part[m] = vq;
-                        part[G::kStates + m] = vk;
-                    } else {
-                        const bool keys_here = (in_warp & 2) != 0;
-                        float v = (keys_here ? vk : vq) +
-                                  __shfl_xor_sync(0xffffffffu, keys_here ? vq : vk, 2 * LPC);
+                const float2 k = make_float2(kq[u].x, kq[u].y), q = make_float2(kq[u].z, kq[u].w);
+                const float2 gh = fma2(q, both(in[u].z), g);
+                g = mul2(decay[u], gh);
+                const float2 moved = mul2(g, h[tb + u]), pk = mul2(gh, k), pa = mul2(moved, rate);
+                dk[u] = mul2(gh, both(in[u].y));
+                grate = fma2(moved, both(in[u].x), grate);
+                out_ka[u] = make_float2(pk.x + pk.y, pa.x + pa.y);
+            }
+            // over the warp's channels: the states' exchange, then queries against keys, then plain sums
 #pragma unroll
-                        for (int off = 4 * LPC; off < 32; off *= 2) v += __shfl_xor_sync(0xffffffffu, v, off);
-                        part[(keys_here ? G::kStates : 0) + m] = v;
-                    }
+            for (int u = 0; u < kBatch; ++u) {
+                const float2 dq = mul2(both(in[u].z), h[tb + u + 1]);
+                if (G::kPerWarp == 1) {
+                    float *part = sh.part[warp][tb + u] + n0;
+                    *reinterpret_cast<float2 *>(part) = dq;
+                    *reinterpret_cast<float2 *>(part + G::kStates) = dk[u];
+                } else {
+                    vqk[u] = make_float2(dq.x + __shfl_xor_sync(0xffffffffu, dq.y, LPC),
+                                         dk[u].x + __shfl_xor_sync(0xffffffffu, dk[u].y, LPC));
                 }
             }
-            lane_sums<kBatch, LPC>(sk, sub);
-            lane_sums<kBatch, LPC>(sa, sub);
-            lane_sums<kBatch, LPC>(sr, sub);
+            if (G::kPerWarp == 2) {
 #pragma unroll
-            for (int i = 0; i < kept_sums<kBatch, LPC>(); ++i) {
-                const int o = (tb + first_sum<kBatch, LPC>(sub) + i) * G::kPitch + c;
-                sh.gk[o] = sk[i];
-                sh.ga[o] = sa[i];
-                sh.r[o] = sr[i];
+                for (int u = 0; u < kBatch; ++u) {
+                    sh.part[warp][tb + u][n0 + m] = vqk[u].x;
+                    sh.part[warp][tb + u][G::kStates + n0 + m] = vqk[u].y;
+                }
+            } else if (G::kPerWarp > 2) {
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u) {
+                    float v = (keys_here ? vqk[u].y : vqk[u].x) +
+                              __shfl_xor_sync(0xffffffffu, keys_here ? vqk[u].x : vqk[u].y, 2 * LPC);
+#pragma unroll
+                    for (int off = 4 * LPC; off < 32; off *= 2) v += __shfl_xor_sync(0xffffffffu, v, off);
+                    sh.part[warp][tb + u][part_at] = v;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                sh.lane_ka[tb + u][tid] = out_ka[u];
+                sh.lane_r[tb + u][tid] = out_r[u];
             }
         }
         __syncthreads();
-        const long at_row = (p.first + t0 + er) * a.channels + cc;
 #pragma unroll
         for (int i = 0; i < kElems; ++i) {
             const int t = er + i * G::kRows;
-            if (own && t < count) {
-                const long r = at_row + i * G::kRows * a.channels;
-                const int o = t * G::kPitch + ec;
-                const float x = sh.x[t][ec], dr = sh.dr[t][ec].x;
-                const float2 slope = sh.slopes[t][ec];
-                const float gd = fmaf(x, sh.gk[o], kLn2 * sh.ga[o]) * slope.x;  // rates were in powers of two
-                static_cast<T *>(a.grad_values)[r] = from_float<T>(fmaf(sh.in[t][ec].x, sh.gk[o], skip * dr));
-                static_cast<T *>(a.grad_steps)[r] = from_float<T>(gd);
+            if (whole || (own && t < count)) {
+                const unsigned r = to_values.offset + i * to_values.step;
+                const float4 in = sh.in[t][ec];
+                const float x = in.w, dr = in.z;
+                const float2 slope = sh.slopes[t][ec], ka = sums_of<LPC>(sh.lane_ka[t], ec);
+                const float gd = fmaf(x, ka.x, kLn2 * ka.y) * slope.x;  // rates were in powers of two
+                to_values.tile[r] = from_float<T>(fmaf(in.x, ka.x, skip * dr));
+                to_steps[r] = from_float<T>(gd);
                 if (a.gate != nullptr)
-                    static_cast<T *>(a.grad_gate)[r] = from_float<T>(slope.y * fmaf(skip, x, sh.r[o]));
+                    to_gate[r] = from_float<T>(slope.y * fmaf(skip, x, sum_of<LPC>(sh.lane_r[t], ec)));
                 gbias += gd;
                 gskip = fmaf(dr, x, gskip);
             }
         }
-        float *key_part = a.key_part + (tile * a.seq.tokens + p.first + t0) * 2 * a.states;
-        for (int i = tid; i < count * 2 * G::kStates; i += kThreads) {
-            const int t = i / (2 * G::kStates), e = i % (2 * G::kStates);
-            float v = 0.f;
+        const bool even = (a.states & 1) == 0;
+        for (int i = tid; i < count * G::kStates; i += kThreads) {  // pairs of [token][2][kStates]
+            const unsigned t = i / G::kStates, e = i % G::kStates * 2, which = e / G::kStates, n = e % G::kStates;
+            float2 v = both(0.f);
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) v += sh.part[w][t][e];
-            const int which = e / G::kStates, n = e % G::kStates;
-            if (n < a.states) key_part[(t * 2 + which) * a.states + n] = v;
+            for (int w = 0; w < kWarps; ++w)
+                v = __fadd2_rn(v, *reinterpret_cast<const float2 *>(&sh.part[w][t][e]));
+            float *o = key_part + (t * 2 + which) * a.states + n;
+            if (even && n < a.states) {
+                *reinterpret_cast<float2 *>(o) = v;
+            } else if (n < a.states) {
+                o[0] = v.x;
+                if (n + 1 < a.states) o[1] = v.y;
+            }
         }
+        to_values.tile += to_values.advance;
+        to_steps += to_values.advance;
+        to_gate += to_values.advance;
+        key_part -= kSegment * 2 * a.states;
         __syncthreads();
     }
     const long entry = p.s * a.chunks + chunk;
@@ -699,8 +854,9 @@ template <typename T, int LPC> __global__ void __launch_bounds__(kThreads) scan_
         const T *q = static_cast<const T *>(a.queries) + s * a.query_stride + col;
         const float2 kk = make_float2(to_float(k[0]), second ? to_float(k[1]) : 0.f);
         const float2 qq = make_float2(to_float(q[0]), second ? to_float(q[1]) : 0.f);
-        if (a.softplus) d = softplus_f(d);
-        h = fma2(decay_of(both(d), mul2(rate, both(kLog2e))), h, mul2(both(d * x), kk));
+        float unused;
+        if (a.softplus) d = softplus_f<false>(d, unused);
+        h = fma2(decay_of(d, mul2(rate, both(kLog2e))), h, mul2(both(d * x), kk));
         const float2 y = mul2(qq, h);
         sum = y.x + y.y;
         store_states(state + row * a.states + n0, n0, 0, a.states, h);
@@ -777,12 +933,15 @@ ScanArgs shape_args(long tokens, long sequences, int channels, int states, int g
 }
 
 template <typename T, int LPC> int launch_forward(const ScanArgs &a, cudaStream_t st) {
+    constexpr int bytes = Geometry<LPC>::kTile * kThreads * static_cast<int>(sizeof(float));
+    if (cudaError_t e = cudaFuncSetAttribute(scan_forward<T, LPC>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes))
+        return fail(BSSM_ERR_CUDA, "selective_scan: %s", cudaGetErrorString(e));
     const dim3 grid(static_cast<unsigned>(a.seq.count * a.tiles), static_cast<unsigned>(a.chunks));
     if (a.chunks > 1) {
         scan_local<T, LPC, false><<<dim3(grid.x, grid.y - 1), kThreads, 0, st>>>(a);
         scan_join<false><<<blocks_for(a.seq.count * a.channels * a.states), kThreads, 0, st>>>(a);
     }
-    scan_forward<T, LPC><<<grid, kThreads, 0, st>>>(a);
+    scan_forward<T, LPC><<<grid, kThreads, bytes, st>>>(a);
     return check_launch("selective_scan");
 }
 template <typename T, int LPC> int launch_backward(const ScanArgs &a, cudaStream_t st) {
