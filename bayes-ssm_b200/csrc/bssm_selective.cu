@@ -72,13 +72,14 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __
 // subnormal results are zero).  The unit cuts its argument's low bits off: measured over d A in [-0.35, -1e-4],
 // where a state remembers many tokens and a bias adds up, its results were 0.10 to 0.37 of 2^-24 low on average,
 // and within -0.11 to 0.16 with 3 * 2^-27 added to the argument, which the multiplication takes along as an FMA.
+constexpr float kExponentBias = 3.f / 134217728.f;
 __device__ __forceinline__ float exp2_unit(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ float2 decay_of(float d, float2 rate) {
-    const float2 e = fma2(both(d), rate, both(3.f / 134217728.f));
+    const float2 e = fma2(both(d), rate, both(kExponentBias));
     return make_float2(exp2_unit(e.x), exp2_unit(e.y));
 }
 
@@ -834,42 +835,125 @@ __global__ void __launch_bounds__(kThreads) scan_sum_rows(const ScanArgs a, floa
     *out = v;
 }
 
-// One token per sequence, the states [sequences][channels][N] moved on in place.
-template <typename T, int LPC> __global__ void __launch_bounds__(kThreads) scan_step(const ScanArgs a, float *state) {
-    const long id = static_cast<long>(blockIdx.x) * kThreads + threadIdx.x;
-    const long row = id / LPC;  // sequence * channels + channel
-    const int sub = static_cast<int>(id % LPC), n0 = 2 * sub;
-    const bool ok = row < a.seq.count * a.channels;
-    const bool live = ok && n0 < a.states, second = n0 + 1 < a.states;
-    const long s = ok ? row / a.channels : 0, c = ok ? row % a.channels : 0;
-    const long col = c / a.group_channels * a.states + n0;
-    float sum = 0.f, x = 0.f;
-    if (live) {
-        x = to_float(static_cast<const T *>(a.values)[s * a.value_stride + c]);
-        float d = to_float(static_cast<const T *>(a.steps)[s * a.step_stride + c]);
-        if (a.step_bias != nullptr) d += a.step_bias[c];
-        float2 h = load_states(state + row * a.states + n0, n0, 0, a.states);
-        const float2 rate = load_states(a.rates + c * a.states + n0, n0, 0, a.states);
-        const T *k = static_cast<const T *>(a.keys) + s * a.key_stride + col;
-        const T *q = static_cast<const T *>(a.queries) + s * a.query_stride + col;
-        const float2 kk = make_float2(to_float(k[0]), second ? to_float(k[1]) : 0.f);
-        const float2 qq = make_float2(to_float(q[0]), second ? to_float(q[1]) : 0.f);
-        float unused;
-        if (a.softplus) d = softplus_f<false>(d, unused);
-        h = fma2(decay_of(d, mul2(rate, both(kLog2e))), h, mul2(both(d * x), kk));
-        const float2 y = mul2(qq, h);
-        sum = y.x + y.y;
-        store_states(state + row * a.states + n0, n0, 0, a.states, h);
-    }
+// One token per sequence, the states [sequences][channels][N] moved on in
+// place: bound by the states' traffic, 8 bytes each.  A lane holds VEC states
+// (4 where N is a multiple of 4: 16-byte accesses) of a channel, LANES lanes (a
+// power of two) the channel; it walks every gridDim.y-th sequence, so that
+// rates and addresses are made once, and loads a sequence ahead.
+template <typename T, int VEC> struct StepKeys {  // VEC adjacent keys on their way: one word each, or packed
+    unsigned w[VEC];
+    __device__ __forceinline__ void load(const T *p, int n, bool wide) {
+        if (sizeof(T) == 2 && VEC > 1 && wide) {
+            const Packed<unsigned, (VEC + 1) / 2> v = load_packed<unsigned, (VEC + 1) / 2>(reinterpret_cast<const unsigned *>(p));
 #pragma unroll
-    for (int off = LPC / 2; off >= 1; off /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    if (live && sub == 0) {
-        if (a.skip != nullptr) sum = fmaf(a.skip[c], x, sum);
-        if (a.gate != nullptr) {
-            const float z = to_float(static_cast<const T *>(a.gate)[s * a.gate_stride + c]);
-            sum *= z * gate_sigmoid<T>(z);
+            for (int j = 0; j < (VEC + 1) / 2; ++j) w[j] = v.e[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                Raw<T> r{0};
+                if (j < n) r.load(p + j);
+                w[j] = r.bits;
+            }
         }
-        static_cast<T *>(a.out)[s * a.channels + c] = from_float<T>(sum);
+    }
+    __device__ __forceinline__ void values(bool wide, float (&o)[VEC]) const {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const unsigned pair = w[j / 2];
+            const unsigned bits = sizeof(T) == 2 && VEC > 1 && wide ? (j % 2 == 0 ? pair & 0xffffu : pair >> 16) : w[j];
+            o[j] = Raw<T>{bits}.value();
+        }
+    }
+};
+
+template <typename T, int VEC, int LANES>
+__global__ void __launch_bounds__(kThreads, 4) scan_step(const ScanArgs a, float *state) {
+    const int sub = threadIdx.x % LANES, n0 = VEC * sub;
+    const int c = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
+    const bool live = c < a.channels && n0 < a.states;
+    const int n = live ? min(VEC, a.states - n0) : 0;
+    const long group = a.groups == 1 ? 0 : c / a.group_channels;
+    const long row = static_cast<long>(a.channels) * a.states, at = static_cast<long>(c) * a.states + n0;
+    // whole vectors everywhere: VEC divides N, and the keys' rows are aligned to it
+    const bool whole = a.states % VEC == 0;
+    const auto aligned = [&](const void *p, long stride) {
+        return whole && stride % VEC == 0 && reinterpret_cast<uintptr_t>(p) % (VEC * sizeof(T)) == 0;
+    };
+    const bool wide_k = aligned(a.keys, a.key_stride), wide_q = aligned(a.queries, a.query_stride);
+    float rate[VEC], bias = 0.f, skip = 0.f;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) rate[j] = j < n ? a.rates[at + j] * kLog2e : 0.f;
+    if (live && a.step_bias != nullptr) bias = a.step_bias[c];
+    if (live && a.skip != nullptr) skip = a.skip[c];
+    long s = blockIdx.y;
+    float *h_at = state + s * row + at;
+    const T *x_at = static_cast<const T *>(a.values) + s * a.value_stride + c;
+    const T *d_at = static_cast<const T *>(a.steps) + s * a.step_stride + c;
+    const T *z_at = static_cast<const T *>(a.gate) + s * a.gate_stride + c;
+    const T *k_at = static_cast<const T *>(a.keys) + s * a.key_stride + group * a.states + n0;
+    const T *q_at = static_cast<const T *>(a.queries) + s * a.query_stride + group * a.states + n0;
+    T *out = static_cast<T *>(a.out) + s * a.channels + c;
+    const long on = gridDim.y;
+    float next_h[VEC];
+    Raw<T> next_x{0}, next_d{0}, next_z{0};
+    StepKeys<T, VEC> next_k{}, next_q{};
+    auto load = [&]() {
+        if (!live) return;
+        if (whole) {
+            const Packed<float, VEC> v = load_packed<float, VEC>(h_at);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) next_h[j] = v.e[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) next_h[j] = j < n ? h_at[j] : 0.f;
+        }
+        next_x.load(x_at);
+        next_d.load(d_at);
+        if (a.gate != nullptr) next_z.load(z_at);
+        next_k.load(k_at, n, wide_k);
+        next_q.load(q_at, n, wide_q);
+        x_at += on * a.value_stride;
+        d_at += on * a.step_stride;
+        z_at += on * a.gate_stride;
+        k_at += on * a.key_stride;
+        q_at += on * a.query_stride;
+    };
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) next_h[j] = 0.f;
+    load();
+    for (; s < a.seq.count; s += on) {
+        float h[VEC], k[VEC], q[VEC], sum = 0.f, unused;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) h[j] = next_h[j];
+        next_k.values(wide_k, k);
+        next_q.values(wide_q, q);
+        const float x = next_x.value(), z = next_z.value();
+        float d = next_d.value() + bias;
+        float *const to = h_at;
+        h_at += on * row;
+        if (s + on < a.seq.count) load();
+        if (a.softplus) d = softplus_f<false>(d, unused);
+        const float in = d * x;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            h[j] = fmaf(exp2_unit(fmaf(d, rate[j], kExponentBias)), h[j], in * k[j]);
+            sum = fmaf(q[j], h[j], sum);
+        }
+        if (live && whole) {
+            store_packed<float, VEC>(to, h);
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (j < n) to[j] = h[j];
+        }
+#pragma unroll
+        for (int off = LANES / 2; off >= 1; off /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if (live && sub == 0) {
+            sum = fmaf(skip, x, sum);
+            if (a.gate != nullptr) sum *= z * gate_sigmoid<T>(z);
+            *out = from_float<T>(sum);
+        }
+        out += on * a.channels;
     }
 }
 
@@ -956,10 +1040,18 @@ template <typename T, int LPC> int launch_backward(const ScanArgs &a, cudaStream
     scan_backward<T, LPC><<<grid, kThreads, bytes, st>>>(a);
     return check_launch("selective_scan_backward");
 }
-template <typename T, int LPC> int launch_step(const ScanArgs &a, cudaStream_t st) {
-    const long threads = a.seq.count * a.channels * LPC;
-    scan_step<T, LPC><<<static_cast<unsigned>((threads + kThreads - 1) / kThreads), kThreads, 0, st>>>(a, a.state1);
+template <typename T, int VEC, int LANES> int launch_step_as(const ScanArgs &a, cudaStream_t st) {
+    // one wave of CTAs, four an SM
+    const long columns = (static_cast<long>(a.channels) * LANES + kThreads - 1) / kThreads;
+    long rows = 592 / columns;
+    rows = rows < 1 ? 1 : rows < a.seq.count ? rows : a.seq.count;
+    const dim3 grid(static_cast<unsigned>(columns), static_cast<unsigned>(rows));
+    scan_step<T, VEC, LANES><<<grid, kThreads, 0, st>>>(a, a.state1);
     return check_launch("selective_step");
+}
+template <typename T, int LPC> int launch_step(const ScanArgs &a, cudaStream_t st) {
+    if (a.states % 4 == 0) return launch_step_as<T, 4, LPC < 2 ? 1 : LPC / 2>(a, st);
+    return launch_step_as<T, 2, LPC>(a, st);
 }
 
 enum ScanKind { kScan, kScanBackward, kScanStep };
