@@ -181,22 +181,22 @@ template <typename T, int VEC, int W> __global__ void __launch_bounds__(kThreads
         float win[W - 1][VEC];
 #pragma unroll
         for (int j = 0; j < W - 1; ++j) load_input<T, VEC, W>(a, s, first, g - (W - 1) + j, c, win[j]);
-        Packed<T, VEC> p[kAhead];
+        RawVec<T, VEC> p[kAhead];
         auto load = [&](long t) {
             if (t + kAhead > last) return;
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) p[k] = load_packed<T, VEC>(x + (t + k) * a.row_stride);
+            for (int k = 0; k < kAhead; ++k) p[k].load(x + (t + k) * a.row_stride);
         };
         load(g);
         for (; g + kAhead <= last; g += kAhead) {
-            Packed<T, VEC> now[kAhead];
+            RawVec<T, VEC> now[kAhead];
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) now[k] = p[k];
             load(g + kAhead);
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
                 float v[VEC];
-                widen(now[k], v);
+                now[k].values(v);
                 emit(g + k, win, v);
                 slide<VEC, W - 1>(win, v);
             }
@@ -320,18 +320,18 @@ template <typename T, int VEC, int W> __global__ void __launch_bounds__(kThreads
         };
         long t = lo;
         for (; t < lo + W - 1 && t < hi + W - 1; ++t) edge(t);
-        Packed<T, VEC> next_x[kAhead], next_g[kAhead];
+        RawVec<T, VEC> next_x[kAhead], next_g[kAhead];
         auto load = [&](long from) {
             if (from + kAhead > hi) return;
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
-                next_x[k] = load_packed<T, VEC>(x + (from + k) * a.row_stride);
-                next_g[k] = load_packed<T, VEC>(gy + (from + k) * a.channels);
+                next_x[k].load(x + (from + k) * a.row_stride);
+                next_g[k].load(gy + (from + k) * a.channels);
             }
         };
         load(t);
         for (; t + kAhead <= hi; t += kAhead) {
-            Packed<T, VEC> px[kAhead], pg[kAhead];
+            RawVec<T, VEC> px[kAhead], pg[kAhead];
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
                 px[k] = next_x[k];
@@ -341,8 +341,8 @@ template <typename T, int VEC, int W> __global__ void __launch_bounds__(kThreads
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
                 float v[VEC], du[VEC];
-                widen(px[k], v);
-                widen(pg[k], du);
+                px[k].values(v);
+                pg[k].values(du);
                 advance(std::true_type{}, t + k, v, du);
             }
         }

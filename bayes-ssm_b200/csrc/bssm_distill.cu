@@ -30,7 +30,9 @@
 namespace bssm {
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kResident = 6;         // CTAs an SM
+constexpr long kStretchBytes = 81920;  // longest stretch of a row that a CTA takes while clusters allow it
 constexpr int kMaxTop = 1024;
 constexpr int kCounters = 148;       // partial counts of the rows with a teacher
 constexpr long kCountHere = 4096;    // entries up to which every CTA counts the rows itself
@@ -49,6 +51,7 @@ struct DistillArgs {
     void *grad;              // null: none
     const float *upstream;   // backward: null is 1
     int upstream_per_row;
+    int words;               // of the bits of a stretch; 0: the stretch is too long for them
 };
 
 __device__ __forceinline__ float exp2_unit(float x) {
@@ -91,17 +94,15 @@ __device__ __forceinline__ int count_rows(const DistillArgs &a, long first, long
     }
     return n;
 }
-__global__ void __launch_bounds__(kThreads) distill_count(const DistillArgs a) {
-    __shared__ int part[kWarps];
+__global__ void __launch_bounds__(1024) distill_count(const DistillArgs a) {
+    __shared__ int part[32];
     const int warp = threadIdx.x / 32;
-    const int n = count_rows(a, blockIdx.x * kWarps + warp, static_cast<long>(kCounters) * kWarps);
+    const int n = count_rows(a, blockIdx.x * 32 + warp, static_cast<long>(kCounters) * 32);
     if (threadIdx.x % 32 == 0) part[warp] = n;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        int total = 0;
-        for (int w = 0; w < kWarps; ++w) total += part[w];
-        a.counts[blockIdx.x] = total;
-    }
+    if (warp != 0) return;
+    const int total = __reduce_add_sync(0xffffffffu, part[threadIdx.x]);
+    if (threadIdx.x == 0) a.counts[blockIdx.x] = total;
 }
 // All rows with a teacher, in every thread of the CTA; `part` is its scratch.
 __device__ __forceinline__ int all_rows(const DistillArgs &a, int *part) {
@@ -138,11 +139,8 @@ template <typename T> struct Stretch {
 };
 
 // One vector into a thread's running maximum and sum.
-template <int VEC> __device__ __forceinline__ void add_vector(const float (&v)[VEC], float scale, float &m, float &f,
-                                                              float2 &s) {
-    float top = fmaxf(v[0], v[1]);
-#pragma unroll
-    for (int e = 2; e < VEC; ++e) top = fmaxf(top, v[e]);
+template <int VEC> __device__ __forceinline__ void add_vector(float top, const float (&v)[VEC], float scale, float &m,
+                                                              float &f, float2 &s) {
     if (top > m) {
         const float g = finite_max(top), by = m == -INFINITY ? 0.f : exp2_unit((m - g) * scale);
         s = make_float2(s.x * by, s.y * by);
@@ -158,13 +156,16 @@ template <int VEC> __device__ __forceinline__ void add_vector(const float (&v)[V
 }
 
 // BACKWARD: the maximum and sum are the forward's.
-template <typename T, bool BACKWARD> __global__ void __launch_bounds__(kThreads, 3) distill_rows(const DistillArgs a) {
+template <typename T, bool BACKWARD>
+__global__ void __launch_bounds__(kThreads, kResident) distill_rows(const DistillArgs a) {
     constexpr int kVec = 16 / sizeof(T);
     __shared__ float p_s[kMaxTop];
     __shared__ __align__(16) int i_s[kMaxTop + 4];
-    __shared__ float2 stat_s[kWarps];
-    __shared__ float2 mine_s;  // this CTA's maximum and sum, read by its cluster
-    __shared__ int count_s[kWarps];
+    __shared__ float2 stat_s[kWarps], teacher_s[kWarps];
+    __shared__ float loss_s[kWarps];
+    __shared__ int bad_s[kWarps], count_s[kWarps], again_s;
+    __shared__ float2 mine_s;           // this CTA's maximum and sum, read by its cluster
+    extern __shared__ unsigned named[]; // a bit for every logit of the stretch: named by the teacher
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = static_cast<int>(cluster.block_rank()), ranks = static_cast<int>(cluster.num_blocks());
@@ -174,22 +175,54 @@ template <typename T, bool BACKWARD> __global__ void __launch_bounds__(kThreads,
     T *grad = a.grad == nullptr ? nullptr : static_cast<T *>(a.grad) + r * a.vocab;
     const Stretch<T> at(row, a.vocab, rank, ranks);
     const float scale = kLog2e / a.temperature;  // exponents in powers of two
+    const bool counters = a.mean && a.rows * a.top > kCountHere;
+    int counted = 0;
+    if (counters)
+        for (int i = lane; i < kCounters; i += 32) counted += a.counts[i];
+    for (int i = tid; i < a.words; i += kThreads) named[i] = 0;
+    if (tid == 0) again_s = 0;
 
     // the teacher's entries; -1 marks an empty one, -2 one past the vocabulary
-    bool any = false;
+    float top = -INFINITY, total = 0.f;
+    bool bad = false;
     for (int k = tid; k < a.top; k += kThreads) {
         const long e = entry_of(a, r * a.top + k);
         const float t = e < 0 ? -INFINITY : load_as_float(a.teacher, a.teacher_dtype, r * a.top + k);
-        any |= t != -INFINITY;
+        const int j = t == -INFINITY ? -1 : e >= a.vocab ? -2 : static_cast<int>(e);
         p_s[k] = t;
-        i_s[k] = t == -INFINITY ? -1 : e >= a.vocab ? -2 : static_cast<int>(e);
+        i_s[k] = j;
+        bad |= j == -2;
+        top = fmaxf(top, j == -1 ? -INFINITY : t);
     }
     if (tid < 4) i_s[a.top + tid] = -1;
-    if (!__syncthreads_or(any)) {  // no teacher
+    const bool any = __any_sync(0xffffffffu, top != -INFINITY);
+    bool nan = false;  // a NaN gives way in fmaxf, but is an entry
+    for (int k = tid; k < a.top; k += kThreads) nan |= p_s[k] != p_s[k];
+    top = warp_max(top);
+    for (int k = tid; k < a.top; k += kThreads) total += exp2f((p_s[k] - finite_max(top)) * scale);
+    total = warp_sum(total);
+    bad = __any_sync(0xffffffffu, bad);
+    if (lane == 0) {
+        teacher_s[warp] = make_float2(top, total);
+        bad_s[warp] = bad;
+    }
+    if (!__syncthreads_or(any || nan)) {  // no teacher
         if (!BACKWARD && tid == 0 && rank == 0) a.row_loss[r] = 0.f;
         if (grad != nullptr)
             for (int j = at.lo + tid; j < at.hi; j += kThreads) grad[j] = from_float<T>(0.f);
         return;  // every CTA of the cluster does
+    }
+    {
+        const float2 w = teacher_s[lane % kWarps];
+        top = warp_max(w.x);
+        total = warp_sum(lane < kWarps ? w.y * exp2f((w.x - finite_max(top)) * scale) : 0.f);
+        bad = __any_sync(0xffffffffu, bad_s[lane % kWarps] != 0);
+    }
+    for (int k = tid; k < a.top; k += kThreads) {
+        const int j = i_s[k] - at.lo;
+        if (a.words == 0 || i_s[k] < at.lo || i_s[k] >= at.hi) continue;
+        const unsigned bit = 1u << (j % 32);
+        if ((atomicOr(&named[j / 32], bit) & bit) != 0) again_s = 1;  // named twice
     }
 
     float2 stat;
@@ -200,36 +233,39 @@ template <typename T, bool BACKWARD> __global__ void __launch_bounds__(kThreads,
         float2 s = make_float2(0.f, 0.f);
         auto one = [&](int j) {
             const float v[2] = {to_float(row[j]), -INFINITY};
-            add_vector<2>(v, scale, m, f, s);
+            add_vector<2>(v[0], v, scale, m, f, s);
         };
         for (int j = at.lo + tid; j < at.body; j += kThreads) one(j);
         for (int j = at.tail() + tid; j < at.hi; j += kThreads) one(j);
         const T *body = row + at.body;
         int i = tid;
         for (; i + 3 * kThreads < at.vecs; i += 4 * kThreads) {
-            Packed<T, kVec> p[4];
+            RawVec<T, kVec> p[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) p[u] = load_packed<T, kVec>(body + (i + u * kThreads) * kVec);
+            for (int u = 0; u < 4; ++u) p[u].load(body + (i + u * kThreads) * kVec);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 float v[kVec];
-                widen(p[u], v);
-                add_vector<kVec>(v, scale, m, f, s);
+                p[u].values(v);
+                add_vector<kVec>(p[u].top(), v, scale, m, f, s);
             }
         }
         for (; i < at.vecs; i += kThreads) {
+            RawVec<T, kVec> p;
             float v[kVec];
-            widen(load_packed<T, kVec>(body + i * kVec), v);
-            add_vector<kVec>(v, scale, m, f, s);
+            p.load(body + i * kVec);
+            p.values(v);
+            add_vector<kVec>(p.top(), v, scale, m, f, s);
         }
         stat = make_float2(m, s.x + s.y);
         float2 all = make_float2(warp_max(m), 0.f);
         all.y = warp_sum(stat.y * exp2_unit((m - finite_max(all.x)) * scale));
         if (lane == 0) stat_s[warp] = all;
         __syncthreads();
-        stat = stat_s[0];
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w) stat = join(stat, stat_s[w], scale);
+        stat = stat_s[lane % kWarps];
+        all.x = warp_max(stat.x);
+        all.y = lane < kWarps ? stat.y * exp2_unit((stat.x - finite_max(all.x)) * scale) : 0.f;
+        stat = make_float2(all.x, warp_sum(all.y));
         if (ranks > 1) {
             if (tid == 0) mine_s = stat;
             cluster.sync();
@@ -240,87 +276,84 @@ template <typename T, bool BACKWARD> __global__ void __launch_bounds__(kThreads,
         if (a.row_stats != nullptr && tid == 0 && rank == 0) a.row_stats[r] = stat;
     }
     // a row of -inf alone has no distribution: m is -inf and what follows is NaN
-    const float m = stat.x, sum = stat.y;
-    // the teacher's softmax, in every warp
-    float top = -INFINITY, total = 0.f;
-    bool bad = false;
-    for (int k = lane; k < a.top; k += 32) {
-        top = fmaxf(top, p_s[k]);
-        bad |= i_s[k] == -2;
-    }
-    const float poison = __any_sync(0xffffffffu, bad) ? NAN : 0.f, inverse = 1.f / sum + poison;
-    top = warp_max(top);
-    for (int k = lane; k < a.top; k += 32) total += exp2f((p_s[k] - top) * scale);
-    total = warp_sum(total);
+    const float m = stat.x, sum = stat.y, poison = bad ? NAN : 0.f, inverse = 1.f / sum + poison;
 
-    if (!BACKWARD && warp == 0 && rank == 0) {
+    if (!BACKWARD && rank == 0) {
         const float log_total = log2f(total), log_sum = log2f(sum);
         float loss = 0.f;
-        for (int k = lane; k < a.top; k += 32) {
+        for (int k = tid; k < a.top; k += kThreads) {
             if (i_s[k] < 0) continue;
             const float lp = (p_s[k] - top) * scale - log_total, p = exp2f(lp);
             const float lq = (to_float(row[i_s[k]]) - m) * scale - log_sum;
             if (p != 0.f) loss = fmaf(p, lp - lq, loss);
         }
         loss = warp_sum(loss);
-        if (lane == 0)
-            a.row_loss[r] = loss * kLn2 * a.temperature * a.temperature + poison + (sum != sum ? NAN : 0.f);
+        if (lane == 0) loss_s[warp] = loss;
     }
-    if (grad == nullptr) return;
     float weight = a.temperature;
-    if (a.upstream != nullptr) weight *= a.upstream[a.upstream_per_row ? r : 0];
-    if (a.mean) weight /= static_cast<float>(max(1, all_rows(a, count_s)));
-    const float factor = weight * inverse;
-    auto one = [&](int j) { grad[j] = from_float<T>(exp2_unit((to_float(row[j]) - m) * scale) * factor); };
-    auto eight = [&](const Packed<T, kVec> &p, float (&v)[kVec]) {
-        widen(p, v);
-#pragma unroll
-        for (int e = 0; e < kVec; e += 2) {
-            const float2 x = __fmul2_rn(__fadd2_rn(make_float2(v[e], v[e + 1]), make_float2(-m, -m)),
-                                        make_float2(scale, scale));
-            const float2 g = __fmul2_rn(make_float2(exp2_unit(x.x), exp2_unit(x.y)), make_float2(factor, factor));
-            v[e] = g.x;
-            v[e + 1] = g.y;
+    if (grad != nullptr) {
+        if (a.upstream != nullptr) weight *= a.upstream[a.upstream_per_row ? r : 0];
+        if (a.mean) {
+            const int n = counters ? __reduce_add_sync(0xffffffffu, counted) : all_rows(a, count_s);
+            weight /= static_cast<float>(max(1, n));
         }
-    };
-    if ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(grad)) % 16 == 0) {
-        for (int j = at.lo + tid; j < at.body; j += kThreads) one(j);
-        for (int j = at.tail() + tid; j < at.hi; j += kThreads) one(j);
-        const T *body = row + at.body;
-        T *out = grad + at.body;
-        int i = tid;
-        for (; i + 3 * kThreads < at.vecs; i += 4 * kThreads) {
-            Packed<T, kVec> p[4];
+        const float factor = weight * inverse;
+        auto one = [&](int j) { grad[j] = from_float<T>(exp2_unit((to_float(row[j]) - m) * scale) * factor); };
+        auto gradients = [&](const RawVec<T, kVec> &p, float (&v)[kVec]) {
+            p.values(v);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) p[u] = load_packed<T, kVec>(body + (i + u * kThreads) * kVec);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                float v[kVec];
-                eight(p[u], v);
-                store_packed<T, kVec>(out + (i + u * kThreads) * kVec, v);
+            for (int e = 0; e < kVec; e += 2) {
+                const float2 x = __fmul2_rn(__fadd2_rn(make_float2(v[e], v[e + 1]), make_float2(-m, -m)),
+                                            make_float2(scale, scale));
+                const float2 g = __fmul2_rn(make_float2(exp2_unit(x.x), exp2_unit(x.y)), make_float2(factor, factor));
+                v[e] = g.x;
+                v[e + 1] = g.y;
             }
+        };
+        if ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(grad)) % 16 == 0) {
+            for (int j = at.lo + tid; j < at.body; j += kThreads) one(j);
+            for (int j = at.tail() + tid; j < at.hi; j += kThreads) one(j);
+            const T *body = row + at.body;
+            T *out = grad + at.body;
+            int i = tid;
+            for (; i + 3 * kThreads < at.vecs; i += 4 * kThreads) {
+                RawVec<T, kVec> p[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) p[u].load(body + (i + u * kThreads) * kVec);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    float v[kVec];
+                    gradients(p[u], v);
+                    store_packed<T, kVec>(out + (i + u * kThreads) * kVec, v);
+                }
+            }
+            for (; i < at.vecs; i += kThreads) {
+                RawVec<T, kVec> p;
+                float v[kVec];
+                p.load(body + i * kVec);
+                gradients(p, v);
+                store_packed<T, kVec>(out + i * kVec, v);
+            }
+        } else {  // rows of logits and gradient fall differently on 16 bytes
+            for (int j = at.lo + tid; j < at.hi; j += kThreads) one(j);
         }
-        for (; i < at.vecs; i += kThreads) {
-            float v[kVec];
-            eight(load_packed<T, kVec>(body + i * kVec), v);
-            store_packed<T, kVec>(out + i * kVec, v);
-        }
-    } else {  // rows of logits and gradient fall differently on 16 bytes
-        for (int j = at.lo + tid; j < at.hi; j += kThreads) one(j);
     }
     __syncthreads();
-    // the entries the teacher names: q - p, the p of an entry named twice added up
+    if (!BACKWARD && tid == 0 && rank == 0) {
+        float loss = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) loss += loss_s[w];
+        a.row_loss[r] = loss * kLn2 * a.temperature * a.temperature + poison + (sum != sum ? NAN : 0.f);
+    }
+    if (grad == nullptr) return;
+    // the entries the teacher names: q - p, the p of an entry named twice added up by the first
     const float per = 1.f / total;
+    const bool again = a.words == 0 || again_s != 0;
     for (int k = tid; k < a.top; k += kThreads) {
         const int j = i_s[k];
         if (j < at.lo || j >= at.hi) continue;
-        int same = 0;
-        for (int o = 0; o < a.top; o += 4) {
-            const int4 i = *reinterpret_cast<const int4 *>(&i_s[o]);
-            same += (i.x == j) + (i.y == j) + (i.z == j) + (i.w == j);
-        }
         float p = exp2f((p_s[k] - top) * scale) * per;
-        if (same > 1) {
+        if (again) {
             bool first = true;
             p = 0.f;
             for (int o = 0; o < a.top; ++o) {
@@ -358,13 +391,21 @@ template <typename T> __global__ void __launch_bounds__(256) distill_scale(T *gr
         grad[i] = from_float<T>(to_float(grad[i]) * f);
 }
 
-template <typename T> int launch_rows(const DistillArgs &a, bool backward, cudaStream_t st) {
-    // Rows alone fill the SMs from 148 on.  Fewer are split, up to a cluster of 8 and 4,096 logits a CTA.
+template <typename T> int launch_rows(DistillArgs a, bool backward, cudaStream_t st) {
+    // Rows alone fill the SMs from 148 on; fewer are split down to 4,096 logits a CTA.  Long ones are split so
+    // that the second pass finds its logits in L2: 6 CTAs an SM of 80 KB are 71 MB.  (8,192 x 32,000 bf16: 215 us,
+    // unsplit; halved 297.  2,048 x 32,000 f32: halved 114, unsplit 133.  2,048 x 128,000 bf16: quarters, 248.)
     int ranks = 1;
-    while (ranks < kMaxCluster && a.rows * ranks * 2 <= 296 && a.vocab / (ranks * 2) >= 4096) ranks *= 2;
+    while (ranks < kMaxCluster &&
+           ((a.rows * ranks * 2 <= 296 && a.vocab / (ranks * 2) >= 4096) ||
+            static_cast<long>(a.vocab) / ranks * static_cast<long>(sizeof(T)) > kStretchBytes))
+        ranks *= 2;
+    const long longest = static_cast<long>(a.vocab) / ranks + 64;  // shares are whole vectors, the ends ragged
+    a.words = longest * static_cast<long>(sizeof(T)) <= 2 * kStretchBytes ? static_cast<int>((longest + 31) / 32) : 0;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(static_cast<unsigned>(a.rows * ranks));
     config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = static_cast<size_t>(a.words) * sizeof(unsigned);
     config.stream = st;
     cudaLaunchAttribute attribute{};
     attribute.id = cudaLaunchAttributeClusterDimension;
@@ -420,7 +461,7 @@ extern "C" int bssm_distillation(const void *logits, int dtype, long rows, int v
     a.temperature = temperature; a.mean = mean; a.counts = counts; a.row_loss = row_loss;
     a.row_stats = reinterpret_cast<float2 *>(row_stats); a.grad = grad;
     if (mean && rows * top > kCountHere) {
-        distill_count<<<kCounters, kThreads, 0, st>>>(a);
+        distill_count<<<kCounters, 1024, 0, st>>>(a);
         if (int rc = check_launch("distillation")) return rc;
     }
     if (rows > 0)

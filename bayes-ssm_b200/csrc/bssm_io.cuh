@@ -8,6 +8,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "bayes_ssm_b200.h"
 
 namespace bssm {
@@ -57,6 +59,57 @@ template <typename T, int VEC> __device__ __forceinline__ void store_packed(T *p
     for (int i = 0; i < VEC; ++i) o.e[i] = from_float<T>(v[i]);
     *reinterpret_cast<Packed<T, VEC> *>(p) = o;
 }
+
+// VEC elements between their load and their use, as whole 32-bit registers.
+// (As 16-bit variables the compiler takes them apart right behind the load,
+// which then waits there instead of running on under other work.)  VEC is a
+// power of two and the address a multiple of min(16, VEC * sizeof(T)).
+template <typename T, int VEC> struct RawVec {
+    static constexpr int kWords = (VEC * static_cast<int>(sizeof(T)) + 3) / 4;
+    unsigned w[kWords];
+
+    __device__ __forceinline__ void load(const T *p) {
+        if constexpr (VEC * sizeof(T) == 2) {
+            w[0] = *reinterpret_cast<const unsigned short *>(p);
+        } else if constexpr (kWords == 1) {
+            w[0] = *reinterpret_cast<const unsigned *>(p);
+        } else if constexpr (kWords == 2) {
+            const uint2 v = *reinterpret_cast<const uint2 *>(p);
+            w[0] = v.x; w[1] = v.y;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWords; i += 4) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(reinterpret_cast<const unsigned *>(p) + i);
+                w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
+            }
+        }
+    }
+    __device__ __forceinline__ float value(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+            return __uint_as_float(i % 2 == 0 ? w[i / 2] << 16 : w[i / 2] & 0xffff0000u);
+        else return __half2float(__ushort_as_half(static_cast<unsigned short>(i % 2 == 0 ? w[i / 2] & 0xffffu : w[i / 2] >> 16)));
+    }
+    __device__ __forceinline__ void values(float (&o)[VEC]) const {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o[i] = value(i);
+    }
+    // The largest (a NaN gives way to a number); 16-bit types two at a time.
+    __device__ __forceinline__ float top() const {
+        if constexpr (sizeof(T) == 4 || VEC == 1) {
+            float m = value(0);
+#pragma unroll
+            for (int i = 1; i < VEC; ++i) m = fmaxf(m, value(i));
+            return m;
+        } else {
+            using T2 = typename std::conditional<std::is_same<T, __nv_bfloat16>::value, __nv_bfloat162, __half2>::type;
+            T2 m = *reinterpret_cast<const T2 *>(&w[0]);
+#pragma unroll
+            for (int i = 1; i < kWords; ++i) m = __hmax2(m, *reinterpret_cast<const T2 *>(&w[i]));
+            return fmaxf(to_float(m.x), to_float(m.y));
+        }
+    }
+};
 
 // expf rather than __expf: the latter rounds x log2 e to float32 first, which
 // costs |x| 2^-24 of the result.

@@ -120,6 +120,22 @@ def test_entries_named_twice_and_narrow_indices(dtype):
     assert rel(torch.autograd.grad(loss, x)[0], torch.autograd.grad(want, x64)[0]) <= TOL[dtype]
 
 
+@pytest.mark.parametrize("level", (-3000.0, 3000.0))
+@pytest.mark.parametrize("top", (3, 40, 700))
+def test_logits_far_from_zero(level, top):
+    """Only differences of logits matter, on either side."""
+    logits, teacher, indices = inputs(3, 3000, top, torch.float32, 15)
+    teacher = teacher + level
+    indices[1, 1:] = -1
+    logits[2] += level
+    want, x64 = reference(logits, teacher, indices, 1.0, "sum")
+    x = logits.requires_grad_()
+    loss = distillation_loss(x, teacher, indices, reduction="sum")
+    # float32 logits of this size are 2^-13 apart, which both sides share
+    assert abs(float(loss.detach()) - float(want.detach())) <= 1e-5 * (3 + abs(float(want.detach())))
+    assert rel(torch.autograd.grad(loss, x)[0], torch.autograd.grad(want, x64)[0]) <= 1e-5
+
+
 def test_teacher_of_another_type():
     logits, teacher, indices = inputs(4, 2000, 6, torch.bfloat16, 8)
     teacher = teacher.float() + 0.01
