@@ -45,6 +45,13 @@ headline, config 3, is ``bench.py``).
 * ``--config d64-profile``: the (64, 64) kernels on 296 chains (B37 T512 H8,
   one wave at two CTAs per SM), untimed: the case their ncu captures run on.
 
+* ``--config selective``: a language model of selective state space blocks
+  (``bayes_ssm.selective_lm``: width 512, 6 layers, inner width 1,024, 16
+  states, MLP 2,048, vocabulary 32,000, BF16): a training step at B8 T2048 from
+  a teacher's 32 top logits a position (tok/s), a 2,048-token prompt of 8
+  sequences, and one token for each of them (us; also replayed as a CUDA
+  graph); beside each, the device time of this package's kernels in it.
+
 * ``--config refcuda``: the reference's own CUDA kernels on the same GPU --
   catid/bayes-ssm installed unmodified into ``baseline/_ref`` (``pip install
   --target``), its D8 extension JIT-built by its own loader
@@ -582,6 +589,45 @@ def envelope_profile(steps: int, warmup: int) -> dict:
             "(profiling case)", "launches": 4 * steps, "timed": False}
 
 
+def selective(steps: int, warmup: int) -> dict:
+    import torch
+
+    from bayes_ssm.selective_lm import SelectiveLM, distill_step
+    from bayes_ssm.six_layer import make_optimizer, parameter_count
+
+    torch.manual_seed(0)
+    b, t, vocab, top = 8, 2048, 32_000, 32
+    model = SelectiveLM(vocab_size=vocab, width=512, layers=6, mlp_width=2048, device="cuda")
+    optimizer = make_optimizer(model)
+    tokens = torch.randint(0, vocab, (b, t), device="cuda")
+    teacher = torch.randn(b, t, top, device="cuda") * 2
+    indices = torch.randint(0, vocab, (b, t, top), device="cuda")
+
+    def train():
+        return distill_step(model, optimizer, tokens, teacher, indices, temperature=2.0)
+
+    def own_ms(fn) -> float:
+        with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+            fn()
+            torch.cuda.synchronize()
+        return sum(e.device_time_total for e in prof.key_averages() if "bssm::" in e.key) / 1e3
+
+    train_ms = _time(train, steps, warmup)
+    prefill_ms = _time(lambda: model.prefill(tokens), steps, warmup)
+    _, state = model.prefill(tokens)
+    one = tokens[:, 0].clone()
+    step_ms = _time(lambda: model.step(one, state), steps, warmup)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        model.step(one, state)
+    graph_ms = _time(graph.replay, steps, warmup)
+    return {"config": "selective", "metric": "tok/s", "value": round(b * t / train_ms * 1e3, 1), "unit": "tok/s",
+            "train_ms": round(train_ms, 3), "train_kernels_ms": round(own_ms(train), 3),
+            "prefill_ms": round(prefill_ms, 3), "prefill_kernels_ms": round(own_ms(lambda: model.prefill(tokens)), 3),
+            "step_us": round(step_ms * 1e3, 1), "step_graph_us": round(graph_ms * 1e3, 1), "step_kernels_us": round(own_ms(lambda: model.step(one, state)) * 1e3, 1),
+            "parameters": parameter_count(model), "batch": b, "tokens": t, "loss": float(train()), "data": "synthetic"}
+
+
 def refcuda64(steps: int, warmup: int) -> dict:
     """The reference's D64 kernels at the ``--config d64`` workload."""
     return refcuda(steps, warmup, key_dim=64)
@@ -701,14 +747,15 @@ def _peak_hbm() -> float:
 def main() -> None:
     ap = argparse.ArgumentParser()
     ap.add_argument("--config", choices=("2", "4", "d64", "d64-profile", "envelope", "envelope-profile", "mixer",
-                                         "refcuda", "refcuda64", "rotation", "rotation-profile"), required=True)
+                                         "refcuda", "refcuda64", "rotation", "rotation-profile", "selective"),
+                    required=True)
     ap.add_argument("--steps", type=int, default=20)
     ap.add_argument("--warmup", type=int, default=3)
     args = ap.parse_args()
     fn = {"2": config2, "4": config4, "d64": d64, "d64-profile": d64_profile, "envelope": envelope,
           "envelope-profile": envelope_profile,
           "mixer": mixer, "refcuda": refcuda, "refcuda64": refcuda64, "rotation": rotation,
-          "rotation-profile": rotation_profile}[args.config]
+          "rotation-profile": rotation_profile, "selective": selective}[args.config]
     print(json.dumps(fn(args.steps, max(3, args.warmup))), flush=True)
 
 
