@@ -370,6 +370,9 @@ template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, 3) sc
         }
         if (left > G::kTile) load(left - G::kTile);
         __syncthreads();
+        const float2 *in_at = &in_s[0][c];
+        const float4 *kq_at = &kq_s[0][sub];
+        float *part_at = part_s + tid;
         for (int tb = 0; tb < count; tb += 8) {
             if (saved != nullptr && (phase + tb) % kSegment == 0) {
                 if (live) store_states(saved, n0, 0, a.states, h);
@@ -379,17 +382,20 @@ template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, 3) sc
             float2 decay[8], inflow[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
-                const float2 in = in_s[tb + u][c], k = *reinterpret_cast<const float2 *>(&kq_s[tb + u][sub]);
+                const float2 in = in_at[u * G::kChannels], k = *reinterpret_cast<const float2 *>(kq_at + u * LPC);
                 decay[u] = decay_of(in.x, rate);
                 inflow[u] = mul2(both(in.y), k);
             }
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
-                const float2 q = *(reinterpret_cast<const float2 *>(&kq_s[tb + u][sub]) + 1);
+                const float2 q = *(reinterpret_cast<const float2 *>(kq_at + u * LPC) + 1);
                 h = fma2(decay[u], h, inflow[u]);
                 const float2 y = mul2(q, h);
-                part_s[(tb + u) * kThreads + tid] = y.x + y.y;
+                part_at[u * kThreads] = y.x + y.y;
             }
+            in_at += 8 * G::kChannels;
+            kq_at += 8 * LPC;
+            part_at += 8 * kThreads;
         }
         __syncthreads();
 #pragma unroll
