@@ -13,7 +13,7 @@
 //
 // The traffic of the logits bounds it: read once, and the gradient written
 // once.  A CTA takes a row (where rows are few, a cluster of CTAs takes one,
-// each a stretch of the vocabulary): a pass for the running maximum and sum,
+// each a stretch of the vocabulary): a pass for the running reference and sum,
 // and, where the gradient is wanted, a second one over logits that are then in
 // L2 (4 rows an SM of 64 to 128 KB are 38 to 76 MB of its 126).  The K entries
 // are corrected afterwards, from the logits again rather than from the rounded
@@ -47,7 +47,7 @@ struct DistillArgs {
     int mean;
     int *counts;             // kCounters partial counts (mean, more than kCountHere entries)
     float *row_loss;         // forward
-    float2 *row_stats;       // (maximum, sum of exp2((s - maximum) log2e / tau)); forward writes, backward reads
+    float2 *row_stats;       // (reference, sum of exp2((s - reference) log2e / tau)); forward writes, backward reads
     void *grad;              // null: none
     const float *upstream;   // backward: null is 1
     int upstream_per_row;
@@ -72,7 +72,7 @@ __device__ __forceinline__ float warp_sum(float v) {
 // The maximum to subtract: where nothing but -inf was seen, any finite one.
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
 
-// Running (maximum, sum) pairs joined: by the larger maximum.
+// Running (reference, sum) pairs joined: by the larger reference.
 __device__ __forceinline__ float2 join(float2 a, float2 b, float scale) {
     const float m = fmaxf(a.x, b.x), f = finite_max(m);
     return make_float2(m, a.y * exp2_unit((a.x - f) * scale) + b.y * exp2_unit((b.x - f) * scale));
@@ -138,24 +138,32 @@ template <typename T> struct Stretch {
     __device__ __forceinline__ int tail() const { return body + vecs * kVec; }
 };
 
-// One vector into a thread's running maximum and sum.
-template <int VEC> __device__ __forceinline__ void add_vector(float top, const float (&v)[VEC], float scale, float &m,
-                                                              float &f, float2 &s) {
-    if (top > m) {
-        const float g = finite_max(top), by = m == -INFINITY ? 0.f : exp2_unit((m - g) * scale);
-        s = make_float2(s.x * by, s.y * by);
-        m = top;
-        f = g;
-    }
-#pragma unroll
-    for (int e = 0; e < VEC; e += 2) {
-        const float2 x = __fmul2_rn(__fadd2_rn(make_float2(v[e], v[e + 1]), make_float2(-f, -f)),
-                                    make_float2(scale, scale));
-        s = __fadd2_rn(s, make_float2(exp2_unit(x.x), exp2_unit(x.y)));
-    }
-}
+// A thread's running sum of exp2((v - reference) log2e / tau).  The reference
+// follows the maximum lazily, once a value is 2^kSlack times its weight above
+// it, so that few vectors rescale the sum: below 2^(17 + kSlack) for any row,
+// far from float32's range.
+constexpr float kSlack = 8.f;
+struct Running {
+    float reference = -INFINITY, shift = 0.f, limit = -INFINITY;  // shift: the reference, or 0 before the first value
+    float2 sum = make_float2(0.f, 0.f);
 
-// BACKWARD: the maximum and sum are the forward's.
+    template <int VEC> __device__ __forceinline__ void add(float top, const float (&v)[VEC], float scale, float slack) {
+        if (top > limit) {
+            const float by = reference == -INFINITY ? 0.f : exp2_unit((reference - top) * scale);
+            sum = make_float2(sum.x * by, sum.y * by);
+            reference = shift = top;
+            limit = top + slack;
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; e += 2) {
+            const float2 x = __fmul2_rn(__fadd2_rn(make_float2(v[e], v[e + 1]), make_float2(-shift, -shift)),
+                                        make_float2(scale, scale));
+            sum = __fadd2_rn(sum, make_float2(exp2_unit(x.x), exp2_unit(x.y)));
+        }
+    }
+};
+
+// BACKWARD: the reference and sum are the forward's.
 template <typename T, bool BACKWARD>
 __global__ void __launch_bounds__(kThreads, kResident) distill_rows(const DistillArgs a) {
     constexpr int kVec = 16 / sizeof(T);
@@ -164,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, kResident) distill_rows(const Distil
     __shared__ float2 stat_s[kWarps], teacher_s[kWarps];
     __shared__ float loss_s[kWarps];
     __shared__ int bad_s[kWarps], count_s[kWarps], again_s;
-    __shared__ float2 mine_s;           // this CTA's maximum and sum, read by its cluster
+    __shared__ float2 mine_s;           // this CTA's reference and sum, read by its cluster
     extern __shared__ unsigned named[]; // a bit for every logit of the stretch: named by the teacher
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
@@ -229,11 +237,11 @@ __global__ void __launch_bounds__(kThreads, kResident) distill_rows(const Distil
     if (BACKWARD) {
         stat = a.row_stats[r];
     } else {
-        float m = -INFINITY, f = 0.f;
-        float2 s = make_float2(0.f, 0.f);
+        Running run;
+        const float slack = kSlack / scale;
         auto one = [&](int j) {
             const float v[2] = {to_float(row[j]), -INFINITY};
-            add_vector<2>(v[0], v, scale, m, f, s);
+            run.add<2>(v[0], v, scale, slack);
         };
         for (int j = at.lo + tid; j < at.body; j += kThreads) one(j);
         for (int j = at.tail() + tid; j < at.hi; j += kThreads) one(j);
@@ -247,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, kResident) distill_rows(const Distil
             for (int u = 0; u < 4; ++u) {
                 float v[kVec];
                 p[u].values(v);
-                add_vector<kVec>(p[u].top(), v, scale, m, f, s);
+                run.add<kVec>(p[u].top(), v, scale, slack);
             }
         }
         for (; i < at.vecs; i += kThreads) {
@@ -255,11 +263,11 @@ __global__ void __launch_bounds__(kThreads, kResident) distill_rows(const Distil
             float v[kVec];
             p.load(body + i * kVec);
             p.values(v);
-            add_vector<kVec>(p.top(), v, scale, m, f, s);
+            run.add<kVec>(p.top(), v, scale, slack);
         }
-        stat = make_float2(m, s.x + s.y);
-        float2 all = make_float2(warp_max(m), 0.f);
-        all.y = warp_sum(stat.y * exp2_unit((m - finite_max(all.x)) * scale));
+        stat = make_float2(run.reference, run.sum.x + run.sum.y);
+        float2 all = make_float2(warp_max(stat.x), 0.f);
+        all.y = warp_sum(stat.y * exp2_unit((stat.x - finite_max(all.x)) * scale));
         if (lane == 0) stat_s[warp] = all;
         __syncthreads();
         stat = stat_s[lane % kWarps];

@@ -418,7 +418,7 @@ template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, 3) sc
 // BACKWARD: the same of the adjoint, which enters at the chunk's end:
 // g -> exp(A D) g + local with g_{t-1} = a_t (q_t dr_t + g_t).
 template <typename T, int LPC, bool BACKWARD>
-__global__ void __launch_bounds__(kThreads, 4) scan_local(const ScanArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) scan_local(const ScanArgs a) {
     using G = Geometry<LPC>;
     __shared__ float2 in_s[G::kTile][G::kChannels];  // (d, d x) or (d, dr)
     __shared__ __align__(16) float k_s[G::kTile * G::kStates];
