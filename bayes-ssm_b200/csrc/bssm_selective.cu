@@ -40,6 +40,7 @@ namespace bssm {
 namespace {
 
 constexpr int kThreads = 256, kWarps = 8;
+constexpr int kChained = 24;  // chunks up to which every one chains those before it itself (a launch saved)
 constexpr int kSegment = 16;  // tokens between the states a forward saves for its backward
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -53,7 +54,7 @@ struct ScanArgs {
     void *out;
     float *state1, *saved;
     // a sequence's chunks of `chunk` tokens (the last to its end), each its own CTA
-    int chunks;
+    int chunks, joined;  // joined: by scan_join, for more than kChained chunks
     long chunk;
     float *carry;  // [sequences][chunks][channels][states]
     float *span;   // [sequences][chunks][channels]: sum of d
@@ -189,6 +190,28 @@ __device__ __forceinline__ void store_states(float *p, int n0, int m, int states
     if (n0 + (1 ^ m) < states) p[1 ^ m] = v.y;
 }
 
+// The state that enters a chunk (BACKWARD: the adjoint, which enters at its
+// end).  A few chunks before (after) it are chained here, from what scan_local
+// found for each; more have been joined by scan_join.
+template <bool BACKWARD>
+__device__ __forceinline__ float2 entering(const ScanArgs &a, long s, int chunk, long c, long at, int n0, int m,
+                                           bool live, float2 rate) {
+    const long row = static_cast<long>(a.channels) * a.states;
+    const float *start = BACKWARD ? a.grad_state1 : a.state0;
+    const int first = BACKWARD ? a.chunks - 1 : 0, step = BACKWARD ? -1 : 1;
+    if (a.joined && chunk != first)
+        return load_states(live ? a.carry + (s * a.chunks + chunk - step) * row + at : nullptr, n0, m, a.states);
+    float2 h = load_states(live && start != nullptr ? start + s * row + at : nullptr, n0, m, a.states);
+#pragma unroll 4
+    for (int k = first; k != chunk; k += step) {
+        const long entry = s * a.chunks + k;
+        const float span = live ? a.span[entry * a.channels + c] : 0.f;
+        const float2 local = load_states(live ? a.carry + entry * row + at : nullptr, n0, m, a.states);
+        h = fma2(make_float2(exp2f(span * rate.x), exp2f(span * rate.y)), h, local);
+    }
+    return h;
+}
+
 // Row of `saved` for token t (a multiple of kSegment) of a sequence: segments
 // of different sequences never share one.
 __device__ __forceinline__ long segment_row(const Sequences &q, long s, long first, long t) {
@@ -300,9 +323,7 @@ template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, 3) sc
     const bool live = c < p.width && n0 < a.states;
     const long row = static_cast<long>(a.channels) * a.states, at = static_cast<long>(p.c0 + c) * a.states + n0;
     const float2 rate = mul2(load_states(live ? a.rates + at : nullptr, n0, 0, a.states), both(kLog2e));
-    const float *start = chunk > 0 ? a.carry + (p.s * a.chunks + chunk - 1) * row
-                         : a.state0 != nullptr ? a.state0 + p.s * row : nullptr;
-    float2 h = load_states(live && start != nullptr ? start + at : nullptr, n0, 0, a.states);
+    float2 h = entering<false>(a, p.s, chunk, p.c0 + c, at, n0, 0, live, rate);
 
     const long row0 = p.first + p.begin;
     Rows<T> values(a.values, a.value_stride, row0, p.c0, er, ec, G::kRows, G::kTile);
@@ -592,9 +613,7 @@ scan_backward(const ScanArgs a) {
     const long row = static_cast<long>(a.channels) * a.states, at = static_cast<long>(p.c0 + c) * a.states + n0;
     const float2 rate = mul2(load_states(live ? a.rates + at : nullptr, n0, m, a.states), both(kLog2e));
     float2 grate = both(0.f);
-    const float *start = chunk < a.chunks - 1 ? a.carry + (p.s * a.chunks + chunk + 1) * row
-                         : a.grad_state1 != nullptr ? a.grad_state1 + p.s * row : nullptr;
-    float2 g = load_states(live && start != nullptr ? start + at : nullptr, n0, m, a.states);
+    float2 g = entering<true>(a, p.s, chunk, p.c0 + c, at, n0, m, live, rate);
     float gskip = 0.f, gbias = 0.f;
 
     const long segments = (p.end - p.begin + kSegment - 1) / kSegment;
@@ -806,32 +825,37 @@ scan_backward(const ScanArgs a) {
     }
 }
 
-// Keys' and queries' gradients: the rows of key_part [tiles][tokens][2][N] of
-// each group's tiles, added in order of the tile.
-template <typename T> __global__ void __launch_bounds__(kThreads) scan_sum_keys(const ScanArgs a, void *grad_keys,
-                                                                                void *grad_queries) {
-    const long cols = a.seq.tokens * 2 * a.states;
+// Everything that the chunks and tiles left in rows, added up in order: keys'
+// and queries' gradients from key_part [tiles][tokens][2][N] (a group's tiles;
+// VEC of N a thread), then rates', skip's and step bias's (the chunks).
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads) scan_sums(const ScanArgs a, void *grad_keys, void *grad_queries,
+                                                      float *grad_rates, float *grad_skip, float *grad_step_bias) {
+    const long cols = a.seq.tokens * 2 * a.states, vecs = cols / VEC * a.groups;
     const long i = static_cast<long>(blockIdx.x) * kThreads + threadIdx.x;
-    if (i >= cols * a.groups) return;
-    const long col = i % cols, group = i / cols;
-    const long token = col / (2 * a.states);
-    const int e = static_cast<int>(col % (2 * a.states)), which = e / a.states, n = e % a.states;
-    float v = 0.f;
-    for (int t = 0; t < a.tiles_per_group; ++t) v += a.key_part[(group * a.tiles_per_group + t) * cols + col];
-    T *out = static_cast<T *>(which == 0 ? grad_queries : grad_keys);
-    out[(token * a.groups + group) * a.states + n] = from_float<T>(v);
-}
-
-// Rates', skip's and step bias's gradients: the chunks' rows added in order.
-__global__ void __launch_bounds__(kThreads) scan_sum_rows(const ScanArgs a, float *grad_rates, float *grad_skip,
-                                                          float *grad_step_bias) {
+    if (i < vecs) {
+        const long group = a.groups == 1 ? 0 : i / (cols / VEC), col = (i - group * (cols / VEC)) * VEC;
+        const long token = col / (2 * a.states);
+        const int e = static_cast<int>(col - token * 2 * a.states), which = e >= a.states, n = e - which * a.states;
+        const float *part = a.key_part + group * a.tiles_per_group * cols + col;
+        float v[VEC] = {};
+#pragma unroll 4
+        for (int t = 0; t < a.tiles_per_group; ++t) {
+            const Packed<float, VEC> p = load_packed<float, VEC>(part + t * cols);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[j] += p.e[j];
+        }
+        T *out = static_cast<T *>(which == 0 ? grad_queries : grad_keys);
+        store_packed<T, VEC>(out + (token * a.groups + group) * a.states + n, v);
+        return;
+    }
     const long state = static_cast<long>(a.channels) * a.states, rows = a.seq.count * a.chunks;
-    const long i = static_cast<long>(blockIdx.x) * kThreads + threadIdx.x;
-    const long j = i - state;  // of 2 * channels: skip, then step bias
+    const long k = i - vecs;
+    const long j = k - state;  // of 2 * channels: skip, then step bias
     if (j >= 2L * a.channels) return;
-    const float *part = j < 0 ? a.rate_part + i : a.channel_part + j;
+    const float *part = j < 0 ? a.rate_part + k : a.channel_part + j;
     const long pitch = j < 0 ? state : 2L * a.channels;
-    float *out = j < 0 ? grad_rates + i
+    float *out = j < 0 ? grad_rates + k
                  : j < a.channels ? (grad_skip == nullptr ? nullptr : grad_skip + j)
                                   : (grad_step_bias == nullptr ? nullptr : grad_step_bias + j - a.channels);
     if (out == nullptr) return;
@@ -991,6 +1015,7 @@ void set_chunks(ScanArgs &a, long longest, int wanted_ctas, long shortest) {
     if (chunks < 2) return;
     a.chunk = ((longest + chunks - 1) / chunks + kSegment * 2 - 1) / (kSegment * 2) * (kSegment * 2);
     a.chunks = static_cast<int>((longest + a.chunk - 1) / a.chunk);
+    a.joined = a.chunks > kChained;
 }
 void set_forward_chunks(ScanArgs &a, long longest) { set_chunks(a, longest, 296, 128); }
 void set_backward_chunks(ScanArgs &a, long longest) { set_chunks(a, longest, 296, 64); }
@@ -1029,7 +1054,7 @@ template <typename T, int LPC> int launch_forward(const ScanArgs &a, cudaStream_
     const dim3 grid(static_cast<unsigned>(a.seq.count * a.tiles), static_cast<unsigned>(a.chunks));
     if (a.chunks > 1) {
         scan_local<T, LPC, false><<<dim3(grid.x, grid.y - 1), kThreads, 0, st>>>(a);
-        scan_join<false><<<blocks_for(a.seq.count * a.channels * a.states), kThreads, 0, st>>>(a);
+        if (a.joined) scan_join<false><<<blocks_for(a.seq.count * a.channels * a.states), kThreads, 0, st>>>(a);
     }
     scan_forward<T, LPC><<<grid, kThreads, bytes, st>>>(a);
     return check_launch("selective_scan");
@@ -1041,7 +1066,7 @@ template <typename T, int LPC> int launch_backward(const ScanArgs &a, cudaStream
     const dim3 grid(static_cast<unsigned>(a.seq.count * a.tiles), static_cast<unsigned>(a.chunks));
     if (a.chunks > 1) {
         scan_local<T, LPC, true><<<dim3(grid.x, grid.y - 1), kThreads, 0, st>>>(a);
-        scan_join<true><<<blocks_for(a.seq.count * a.channels * a.states), kThreads, 0, st>>>(a);
+        if (a.joined) scan_join<true><<<blocks_for(a.seq.count * a.channels * a.states), kThreads, 0, st>>>(a);
     }
     scan_backward<T, LPC><<<grid, kThreads, bytes, st>>>(a);
     return check_launch("selective_scan_backward");
@@ -1083,6 +1108,21 @@ int launch_scan(ScanKind kind, int dtype, const ScanArgs &a, cudaStream_t st) {
         case BSSM_BF16: return launch_lanes<__nv_bfloat16>(kind, a, st);
         default: return launch_lanes<__half>(kind, a, st);
     }
+}
+
+template <typename T>
+void launch_sums_of(const ScanArgs &a, void *gk, void *gq, float *ga, float *gs, float *gb, cudaStream_t st) {
+    const uintptr_t bits = reinterpret_cast<uintptr_t>(gk) | reinterpret_cast<uintptr_t>(gq);
+    const long keys = a.seq.tokens * 2 * a.states * a.groups, rest = static_cast<long>(a.channels) * (a.states + 2);
+    if (a.states % 4 == 0 && bits % (4 * sizeof(T)) == 0)
+        scan_sums<T, 4><<<blocks_for(keys / 4 + rest), kThreads, 0, st>>>(a, gk, gq, ga, gs, gb);
+    else
+        scan_sums<T, 1><<<blocks_for(keys + rest), kThreads, 0, st>>>(a, gk, gq, ga, gs, gb);
+}
+void launch_sums(int dtype, const ScanArgs &a, void *gk, void *gq, float *ga, float *gs, float *gb, cudaStream_t st) {
+    if (dtype == BSSM_F32) launch_sums_of<float>(a, gk, gq, ga, gs, gb, st);
+    else if (dtype == BSSM_BF16) launch_sums_of<__nv_bfloat16>(a, gk, gq, ga, gs, gb, st);
+    else launch_sums_of<__half>(a, gk, gq, ga, gs, gb, st);
 }
 
 int check_scan(const char *what, int dtype, int channels, int states, int groups, long sequences, long tokens,
@@ -1203,16 +1243,7 @@ extern "C" int bssm_selective_scan_backward(
         return fail(BSSM_ERR_WORKSPACE, "selective_scan_backward: workspace too small");
     if (sequences > 0)
         if (int rc = launch_scan(kScanBackward, dtype, a, st)) return rc;
-    const long cols = tokens * 2 * states * groups;
-    if (cols > 0) {
-        const unsigned grid = blocks_for(cols);
-        if (dtype == BSSM_F32) scan_sum_keys<float><<<grid, kThreads, 0, st>>>(a, grad_keys, grad_queries);
-        else if (dtype == BSSM_BF16) scan_sum_keys<__nv_bfloat16><<<grid, kThreads, 0, st>>>(a, grad_keys, grad_queries);
-        else scan_sum_keys<__half><<<grid, kThreads, 0, st>>>(a, grad_keys, grad_queries);
-    }
-    // rates', then skip's and step bias's rows added up, in one launch
-    const long state = static_cast<long>(channels) * states;
-    scan_sum_rows<<<blocks_for(state + 2L * channels), kThreads, 0, st>>>(a, grad_rates, grad_skip, grad_step_bias);
+    launch_sums(dtype, a, grad_keys, grad_queries, grad_rates, grad_skip, grad_step_bias, st);
     return check_launch("selective_scan_backward");
 }
 

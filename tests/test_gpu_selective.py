@@ -219,6 +219,41 @@ def test_scan_forward_and_gradients(shape, c, n, groups, parts, dtype):
             close(a, b, tol, f"grad {name}")
 
 
+@pytest.mark.parametrize("shape,c,n", [((1, 3400), 24, 16), ([3300, 0, 130, 1700, 1], 40, 6), ((2, 700), 33, 16)])
+def test_scan_long_axis_split(shape, c, n):
+    """Few channels and many tokens: the axis is split over many CTAs, chained
+    by each of them (a few chunks) or by a launch of its own (more than 24, as
+    in the first two), in both directions.  A state remembers 1 / (0.05 d) of
+    these tokens at most, a few hundred, so the tolerance is that of the shorter
+    cases."""
+    i, lengths = scan_inputs(shape, c, n, 1, torch.float32, 31)
+    seqs = None if lengths is None else PackedSequences(lengths, device="cuda")
+    r = dict(zip(NAMES, leaves64(*(i[k] for k in NAMES))))
+    k = dict(zip(NAMES, leaves(*(i[k] for k in NAMES))))
+    want, want_final = call_plain(r, True, lengths)
+    y, final = call(k, True, seqs)
+    close(y, want, 2e-5, "read")
+    close(final, want_final, 2e-5, "final state")
+    g = gen(32)
+    gy, gf = rand(g, *y.shape), rand(g, *final.shape)
+    got = grads((y, final), (gy, gf), [k[n_] for n_ in NAMES])
+    ref = grads((want, want_final), (gy.double(), gf.double()), [r[n_] for n_ in NAMES])
+    for name, a, b in zip(NAMES, got, ref):
+        close(a, b, 2e-5, f"grad {name}")
+
+
+def test_a_step_of_zero_keeps_the_state():
+    """Exactly: the decay of a zero step is 1, also with the exponent's bias."""
+    i, _ = scan_inputs((2, 33), 40, 16, 1, torch.float32, 33)
+    i["steps"].zero_()
+    i["step_bias"] = None
+    _, final = call(i, False, None)
+    assert torch.equal(final, i["state"])
+    selective_step(i["values"][:, 0], i["steps"][:, 0], i["rates"], i["keys"][:, 0], i["queries"][:, 0], final,
+                   skip=i["skip"])
+    assert torch.equal(final, i["state"])
+
+
 def test_scan_gradients_against_differences():
     """<grad, direction> of the kernels against central differences of the
     plain form along random directions of every input."""
