@@ -119,8 +119,15 @@ template <int LPC> struct Geometry {
     static constexpr int kPairs = (kTile * LPC + kThreads - 1) / kThreads;  // pairs of states a thread loads
 };
 
+// Lanes.  In the forward adjacent lanes hold different channels and the same
+// states: shared loads of 8 or 16 bytes take half the wavefronts where lanes
+// 2 i and 2 i + 1 read the same address, and keys and queries are more bytes than
+// a channel's (d, d x) (5 wavefronts a token become 4: 199 -> 193 us).  In the
+// backward, which reads 16 bytes of a channel, adjacent lanes hold different
+// states of one (the other way round it took 528 us against 514).
+//
 // Sums over a channel's lanes go through shared memory: every lane leaves its
-// term at [token][thread], and the thread that finishes the element adds the
+// term at [token][channel][lane], and the thread that finishes the element adds the
 // LPC neighbours (a store per token and a few wide loads per element; exchanges
 // between the lanes would take a shuffle, an add and two selects a token).  The
 // 16-byte loads of 8 neighbouring elements start at different vectors, so that
@@ -319,7 +326,7 @@ template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, 3) sc
     const float bias = own && a.step_bias != nullptr ? a.step_bias[cc] : 0.f;
     const float skip = own && a.skip != nullptr ? a.skip[cc] : 0.f;
     // scan: channel c, states n0 and n0 + 1
-    const int sub = lane % LPC, c = tid / 32 * G::kPerWarp + lane / LPC, n0 = 2 * sub;
+    const int sub = lane / G::kPerWarp, c = tid / 32 * G::kPerWarp + lane % G::kPerWarp, n0 = 2 * sub;
     const bool live = c < p.width && n0 < a.states;
     const long row = static_cast<long>(a.channels) * a.states, at = static_cast<long>(p.c0 + c) * a.states + n0;
     const float2 rate = mul2(load_states(live ? a.rates + at : nullptr, n0, 0, a.states), both(kLog2e));
@@ -393,7 +400,7 @@ template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, 3) sc
         __syncthreads();
         const float2 *in_at = &in_s[0][c];
         const float4 *kq_at = &kq_s[0][sub];
-        float *part_at = part_s + tid;
+        float *part_at = part_s + c * LPC + sub;
         for (int tb = 0; tb < count; tb += 8) {
             if (saved != nullptr && (phase + tb) % kSegment == 0) {
                 if (live) store_states(saved, n0, 0, a.states, h);
@@ -450,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, 3) scan_local(const ScanArgs a) {
     const bool own = ec < p.width;
     const long cc = p.c0 + ec;
     const float bias = own && a.step_bias != nullptr ? a.step_bias[cc] : 0.f;
-    const int sub = lane % LPC, c = tid / 32 * G::kPerWarp + lane / LPC, n0 = 2 * sub;
+    const int sub = lane / G::kPerWarp, c = tid / 32 * G::kPerWarp + lane % G::kPerWarp, n0 = 2 * sub;
     const bool live = c < p.width && n0 < a.states;
     const long row = static_cast<long>(a.channels) * a.states, at = static_cast<long>(p.c0 + c) * a.states + n0;
     const float2 rate = mul2(load_states(live ? a.rates + at : nullptr, n0, 0, a.states), both(kLog2e));
@@ -593,7 +600,7 @@ scan_backward(const ScanArgs a) {
     using S = BackwardShared<LPC>;
     constexpr int kElems = (kSegment * G::kChannels + kThreads - 1) / kThreads;
     constexpr int kPairs = (kSegment * LPC + kThreads - 1) / kThreads;
-    constexpr int kBatch = 4;  // tokens between which loads are kept apart
+    constexpr int kBatch = 8;  // tokens between which loads are kept apart (4: 528 us, 2: 546, against 514)
     extern __shared__ __align__(16) unsigned char raw[];
     S &sh = *reinterpret_cast<S *>(raw);
     const long tile = blockIdx.x % a.tiles;
