@@ -576,7 +576,8 @@ template <int LPC> struct BackwardShared {
     static constexpr int kCopies = G::kPerWarp >= 2 ? 2 : 1;
     float4 in[kSegment][G::kChannels];      // d, d x, dr, x
     float2 slopes[kSegment][G::kChannels];  // d's slope in the step, dy silu'(z)
-    float4 kq[kSegment][kCopies][LPC];      // (k, k, q, q) of a lane's states, in either order j ^ m
+    // (k, k, q, q) of a lane's states, then (q, q, k, k) in the other order: both orders' keys in different banks
+    float4 kq[kSegment][kCopies][LPC];
     float2 lane_ka[kSegment][kThreads];     // g . k and g . (A a h) of a lane's states
     float lane_r[kSegment][kThreads];       // q . h
     float part[kWarps][kSegment][2 * G::kStates];
@@ -688,7 +689,7 @@ scan_backward(const ScanArgs a) {
             if (kSegment * LPC % kThreads == 0 || e < kSegment * LPC) {
                 const float2 k = next_k[i].value(paired_k), q = next_q[i].value(paired_q);
                 sh.kq[t][0][n] = make_float4(k.x, k.y, q.x, q.y);
-                if (S::kCopies == 2) sh.kq[t][S::kCopies - 1][n] = make_float4(k.y, k.x, q.y, q.x);
+                if (S::kCopies == 2) sh.kq[t][S::kCopies - 1][n] = make_float4(q.y, q.x, k.y, k.x);
             }
         }
         float2 h[kSegment + 1];  // h[t] before token t of the segment, h[t + 1] after it
@@ -702,7 +703,7 @@ scan_backward(const ScanArgs a) {
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 const float2 in = *reinterpret_cast<const float2 *>(&sh.in[tb + u][c]);
-                const float2 k = *reinterpret_cast<const float2 *>(&sh.kq[tb + u][copy][sub]);
+                const float2 k = reinterpret_cast<const float2 *>(&sh.kq[tb + u][copy][sub])[copy];
                 decay[u] = decay_of(in.x, rate);
                 inflow[u] = mul2(both(in.y), k);
             }
@@ -712,28 +713,28 @@ scan_backward(const ScanArgs a) {
 #pragma unroll
         for (int tb = kSegment - kBatch; tb >= 0; tb -= kBatch) {
             asm volatile("" ::: "memory");  // keeps the compiler from loading later batches early, which spills
-            float4 in[kBatch], kq[kBatch];
-            float2 decay[kBatch], out_ka[kBatch], vqk[kBatch];
+            float4 in[kBatch];
+            float2 k[kBatch], q[kBatch], decay[kBatch], out_ka[kBatch], vqk[kBatch];
             float out_r[kBatch];
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
                 in[u] = sh.in[tb + u][c];
-                kq[u] = sh.kq[tb + u][copy][sub];
+                k[u] = reinterpret_cast<const float2 *>(&sh.kq[tb + u][copy][sub])[copy];
+                q[u] = reinterpret_cast<const float2 *>(&sh.kq[tb + u][copy][sub])[1 - copy];
             }
             // what does not depend on the adjoint first
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
                 decay[u] = decay_of(in[u].x, rate);
-                const float2 pr = mul2(make_float2(kq[u].z, kq[u].w), h[tb + u + 1]);
+                const float2 pr = mul2(q[u], h[tb + u + 1]);
                 out_r[u] = pr.x + pr.y;
             }
             float2 dk[kBatch];
 #pragma unroll
             for (int u = kBatch - 1; u >= 0; --u) {
-                const float2 k = make_float2(kq[u].x, kq[u].y), q = make_float2(kq[u].z, kq[u].w);
-                const float2 gh = fma2(q, both(in[u].z), g);
+                const float2 gh = fma2(q[u], both(in[u].z), g);
                 g = mul2(decay[u], gh);
-                const float2 moved = mul2(g, h[tb + u]), pk = mul2(gh, k), pa = mul2(moved, rate);
+                const float2 moved = mul2(g, h[tb + u]), pk = mul2(gh, k[u]), pa = mul2(moved, rate);
                 dk[u] = mul2(gh, both(in[u].y));
                 grate = fma2(moved, both(in[u].x), grate);
                 out_ka[u] = make_float2(pk.x + pk.y, pa.x + pa.y);
