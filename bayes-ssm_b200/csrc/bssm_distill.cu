@@ -105,18 +105,18 @@ __global__ void __launch_bounds__(1024) distill_count(const DistillArgs a) {
     if (threadIdx.x == 0) a.counts[blockIdx.x] = total;
 }
 // All rows with a teacher, in every thread of the CTA; `part` is its scratch.
-__device__ __forceinline__ int all_rows(const DistillArgs &a, int *part) {
+template <int WARPS> __device__ __forceinline__ int all_rows(const DistillArgs &a, int *part) {
     int n = 0;
     if (a.rows * a.top > kCountHere) {
         for (int i = threadIdx.x % 32; i < kCounters; i += 32) n += a.counts[i];
         return __reduce_add_sync(0xffffffffu, n);
     }
-    n = count_rows(a, threadIdx.x / 32, kWarps);
+    n = count_rows(a, threadIdx.x / 32, WARPS);
     if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = n;
     __syncthreads();
     n = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) n += part[w];
+    for (int w = 0; w < WARPS; ++w) n += part[w];
     return n;
 }
 
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, kResident) distill_rows(const Distil
     if (grad != nullptr) {
         if (a.upstream != nullptr) weight *= a.upstream[a.upstream_per_row ? r : 0];
         if (a.mean) {
-            const int n = counters ? __reduce_add_sync(0xffffffffu, counted) : all_rows(a, count_s);
+            const int n = counters ? __reduce_add_sync(0xffffffffu, counted) : all_rows<kWarps>(a, count_s);
             weight /= static_cast<float>(max(1, n));
         }
         const float factor = weight * inverse;
@@ -376,19 +376,20 @@ __global__ void __launch_bounds__(kThreads, kResident) distill_rows(const Distil
 }
 
 // The rows' losses added in a fixed order, and divided by the rows counted.
-__global__ void __launch_bounds__(kThreads) distill_total(const DistillArgs a, float *loss) {
-    __shared__ float part[kWarps];
-    __shared__ int count_s[kWarps];
+constexpr int kTotalThreads = 1024;
+__global__ void __launch_bounds__(kTotalThreads) distill_total(const DistillArgs a, float *loss) {
+    __shared__ float part[kTotalThreads / 32];
+    __shared__ int count_s[kTotalThreads / 32];
     float v = 0.f;
-    for (long r = threadIdx.x; r < a.rows; r += kThreads) v += a.row_loss[r];
+#pragma unroll 8
+    for (long r = threadIdx.x; r < a.rows; r += kTotalThreads) v += a.row_loss[r];
     v = warp_sum(v);
     if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = v;
+    const int n = a.mean ? all_rows<kTotalThreads / 32>(a, count_s) : 1;
     __syncthreads();
-    const int n = a.mean ? all_rows(a, count_s) : 1;
-    if (threadIdx.x != 0) return;
-    v = 0.f;
-    for (int w = 0; w < kWarps; ++w) v += part[w];
-    *loss = v / static_cast<float>(max(1, n));
+    if (threadIdx.x >= 32) return;
+    v = warp_sum(part[threadIdx.x]);
+    if (threadIdx.x == 0) *loss = v / static_cast<float>(max(1, n));
 }
 
 // grad *= *factor, nothing at all where it is 1 (the loss was the end of the graph).
@@ -475,7 +476,7 @@ extern "C" int bssm_distillation(const void *logits, int dtype, long rows, int v
     if (rows > 0)
         if (int rc = launch_rows(dtype, a, false, st)) return rc;
     if (loss == nullptr) return BSSM_OK;
-    distill_total<<<1, kThreads, 0, st>>>(a, loss);
+    distill_total<<<1, kTotalThreads, 0, st>>>(a, loss);
     return check_launch("distillation");
 }
 
