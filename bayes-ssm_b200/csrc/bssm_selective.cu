@@ -308,6 +308,11 @@ template <typename T> __device__ __forceinline__ bool keys_paired(const void *p,
 }
 
 // The next tile's rows are loaded while this one is scanned.
+// bf16, N16, gate and skip: B8 T2048 C1024 with saved states 193 us (1.0 TB/s;
+// 1.4e12 exponentials a second of 4.5e12), 24 ragged prompts C2048 316 us, the
+// 9 chunks of B1 T8192 C1024 85 us.  Bound by issue slots (57 to 64 % used) and
+// by what 16 to 24 warps an SM wait for; two adjacent channels a thread around
+// the scan (half the loads and stores there) changed these by -3, +4 and -3 us.
 template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, 3) scan_forward(const ScanArgs a) {
     using G = Geometry<LPC>;
     __shared__ float2 in_s[G::kTile][G::kChannels];  // (d, d x)
@@ -445,6 +450,8 @@ template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, 3) sc
 // scan from a state of zero, its outputs left out, and the sum D of its steps.
 // BACKWARD: the same of the adjoint, which enters at the chunk's end:
 // g -> exp(A D) g + local with g_{t-1} = a_t (q_t dr_t + g_t).
+// B1 T8192 C1024 N16 bf16, 9 chunks: 58 us, the exp2 unit at 52 %, the rest of
+// the time waits of 16 warps an SM (two tiles in flight: 58.7 us against 56.8).
 template <typename T, int LPC, bool BACKWARD>
 __global__ void __launch_bounds__(kThreads, 3) scan_local(const ScanArgs a) {
     using G = Geometry<LPC>;
@@ -595,6 +602,10 @@ template <int LPC> struct BackwardShared {
 // A lane holds its two states in the order j ^ m, m the lowest bit that tells
 // the warp's channels apart.  The two halves of the exchange over that bit then
 // are the same registers in every lane and need no selects.
+//
+// B8 T2048 C1024 N16 bf16, gate and skip: 497 us, 1.1e12 exponentials a second
+// of 4.5e12.  Bound by issue slots (50 %) and by shared memory's latency and
+// queue: 128 registers leave 16 warps an SM.
 template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, LPC < 4 ? 1 : 2)
 scan_backward(const ScanArgs a) {
     using G = Geometry<LPC>;
@@ -877,7 +888,9 @@ __global__ void __launch_bounds__(kThreads) scan_sums(const ScanArgs a, void *gr
 // place: bound by the states' traffic, 8 bytes each.  A lane holds VEC states
 // (4 where N is a multiple of 4: 16-byte accesses) of a channel, LANES lanes (a
 // power of two) the channel; it walks every gridDim.y-th sequence, so that
-// rates and addresses are made once, and loads a sequence ahead.
+// rates and addresses are made once (77 -> 32 us), and loads a sequence ahead.
+// B256 C4096 N16 bf16: 32 us for 143 MB, 4.4 TB/s, issue slots 72 % used; B1
+// C1024 N16: 2.0 us, a launch's own time.
 template <typename T, int VEC> struct StepKeys {  // VEC adjacent keys on their way: one word each, or packed
     unsigned w[VEC];
     __device__ __forceinline__ void load(const T *p, int n, bool wide) {
