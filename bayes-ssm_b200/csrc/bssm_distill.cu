@@ -165,7 +165,7 @@ struct Running {
 
 // BACKWARD: the reference and sum are the forward's.
 // 8,192 x 32,000 bf16, K 64, loss and gradient: 204 us for 1.05 GB (5.1 TB/s,
-// 0.80 of a copy's rate; the exp2 unit at 63 %); 2,048 x 32,000 f32, K 32: 112
+// 0.80 of a copy's rate; the exp2 unit at 59 %); 2,048 x 32,000 f32, K 32: 112
 // us (4.7 TB/s); 4 x 50,001 bf16 in clusters of 8: 10 us.  Rows of a few hundred
 // logits cost a CTA's round trips (65,536 x 256: 458 us, 7 ns a row).
 template <typename T, bool BACKWARD>

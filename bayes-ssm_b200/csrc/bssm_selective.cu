@@ -310,7 +310,7 @@ template <typename T> __device__ __forceinline__ bool keys_paired(const void *p,
 // The next tile's rows are loaded while this one is scanned.
 // bf16, N16, gate and skip: B8 T2048 C1024 with saved states 193 us (1.0 TB/s;
 // 1.4e12 exponentials a second of 4.5e12), 24 ragged prompts C2048 316 us, the
-// 9 chunks of B1 T8192 C1024 85 us.  Bound by issue slots (57 to 64 % used) and
+// 9 chunks of B1 T8192 C1024 85 us.  Bound by issue slots (58 to 64 % used) and
 // by what 16 to 24 warps an SM wait for; two adjacent channels a thread around
 // the scan (half the loads and stores there) changed these by -3, +4 and -3 us.
 template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, 3) scan_forward(const ScanArgs a) {
@@ -450,7 +450,7 @@ template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, 3) sc
 // scan from a state of zero, its outputs left out, and the sum D of its steps.
 // BACKWARD: the same of the adjoint, which enters at the chunk's end:
 // g -> exp(A D) g + local with g_{t-1} = a_t (q_t dr_t + g_t).
-// B1 T8192 C1024 N16 bf16, 9 chunks: 58 us, the exp2 unit at 52 %, the rest of
+// B1 T8192 C1024 N16 bf16, 9 chunks: 58 us, the exp2 unit at 51 %, the rest of
 // the time waits of 16 warps an SM (two tiles in flight: 58.7 us against 56.8).
 template <typename T, int LPC, bool BACKWARD>
 __global__ void __launch_bounds__(kThreads, 3) scan_local(const ScanArgs a) {
@@ -604,7 +604,7 @@ template <int LPC> struct BackwardShared {
 // are the same registers in every lane and need no selects.
 //
 // B8 T2048 C1024 N16 bf16, gate and skip: 497 us, 1.1e12 exponentials a second
-// of 4.5e12.  Bound by issue slots (50 %) and by shared memory's latency and
+// of 4.5e12.  Bound by issue slots (54 %) and by shared memory's latency and
 // queue: 128 registers leave 16 warps an SM.
 template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, LPC < 4 ? 1 : 2)
 scan_backward(const ScanArgs a) {
