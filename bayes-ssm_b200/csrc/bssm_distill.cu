@@ -30,12 +30,13 @@
 namespace bssm {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kResident = 6;         // CTAs an SM
+constexpr int kThreadsAnSM = 1536;  // 6 CTAs of 256 threads, 12 of 128 or 24 of 64
 constexpr long kStretchBytes = 81920;  // longest stretch of a row that a CTA takes while clusters allow it
 constexpr int kMaxTop = 1024;
 constexpr int kCounters = 148;       // partial counts of the rows with a teacher
-constexpr long kCountHere = 4096;    // entries up to which every CTA counts the rows itself
+// rows and entries up to which every CTA counts the rows with a teacher itself: a launch saved, and two warps take a
+// microsecond for every two rows
+constexpr long kCountRows = 16, kCountEntries = 4096;
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -45,7 +46,7 @@ struct DistillArgs {
     int vocab, top, teacher_dtype, wide_indices;
     float temperature;
     int mean;
-    int *counts;             // kCounters partial counts (mean, more than kCountHere entries)
+    int *counts;             // kCounters partial counts (a mean's, null where every CTA counts itself)
     float *row_loss;         // forward
     float2 *row_stats;       // (reference, sum of exp2((s - reference) log2e / tau)); forward writes, backward reads
     void *grad;              // null: none
@@ -107,7 +108,7 @@ __global__ void __launch_bounds__(1024) distill_count(const DistillArgs a) {
 // All rows with a teacher, in every thread of the CTA; `part` is its scratch.
 template <int WARPS> __device__ __forceinline__ int all_rows(const DistillArgs &a, int *part) {
     int n = 0;
-    if (a.rows * a.top > kCountHere) {
+    if (a.counts != nullptr) {
         for (int i = threadIdx.x % 32; i < kCounters; i += 32) n += a.counts[i];
         return __reduce_add_sync(0xffffffffu, n);
     }
@@ -167,10 +168,10 @@ struct Running {
 // 8,192 x 32,000 bf16, K 64, loss and gradient: 204 us for 1.05 GB (5.1 TB/s,
 // 0.80 of a copy's rate; the exp2 unit at 59 %); 2,048 x 32,000 f32, K 32: 112
 // us (4.7 TB/s); 4 x 50,001 bf16 in clusters of 8: 10 us.  Rows of a few hundred
-// logits cost a CTA's round trips (65,536 x 256: 458 us, 7 ns a row).
-template <typename T, bool BACKWARD>
-__global__ void __launch_bounds__(kThreads, kResident) distill_rows(const DistillArgs a) {
-    constexpr int kVec = 16 / sizeof(T);
+// logits are bound by their chain of round trips (65,536 x 256: 159 us, 2.4 ns a row).
+template <typename T, bool BACKWARD, int THREADS>
+__global__ void __launch_bounds__(THREADS, kThreadsAnSM / THREADS) distill_rows(const DistillArgs a) {
+    constexpr int kVec = 16 / sizeof(T), kWarps = THREADS / 32;
     __shared__ float p_s[kMaxTop];
     __shared__ __align__(16) int i_s[kMaxTop + 4];
     __shared__ float2 stat_s[kWarps], teacher_s[kWarps];
@@ -187,17 +188,17 @@ __global__ void __launch_bounds__(kThreads, kResident) distill_rows(const Distil
     T *grad = a.grad == nullptr ? nullptr : static_cast<T *>(a.grad) + r * a.vocab;
     const Stretch<T> at(row, a.vocab, rank, ranks);
     const float scale = kLog2e / a.temperature;  // exponents in powers of two
-    const bool counters = a.mean && a.rows * a.top > kCountHere;
+    const bool counters = a.counts != nullptr;
     int counted = 0;
     if (counters)
         for (int i = lane; i < kCounters; i += 32) counted += a.counts[i];
-    for (int i = tid; i < a.words; i += kThreads) named[i] = 0;
+    for (int i = tid; i < a.words; i += THREADS) named[i] = 0;
     if (tid == 0) again_s = 0;
 
     // the teacher's entries; -1 marks an empty one, -2 one past the vocabulary
     float top = -INFINITY, total = 0.f;
     bool bad = false;
-    for (int k = tid; k < a.top; k += kThreads) {
+    for (int k = tid; k < a.top; k += THREADS) {
         const long e = entry_of(a, r * a.top + k);
         const float t = e < 0 ? -INFINITY : load_as_float(a.teacher, a.teacher_dtype, r * a.top + k);
         const int j = t == -INFINITY ? -1 : e >= a.vocab ? -2 : static_cast<int>(e);
@@ -209,9 +210,9 @@ __global__ void __launch_bounds__(kThreads, kResident) distill_rows(const Distil
     if (tid < 4) i_s[a.top + tid] = -1;
     const bool any = __any_sync(0xffffffffu, top != -INFINITY);
     bool nan = false;  // a NaN gives way in fmaxf, but is an entry
-    for (int k = tid; k < a.top; k += kThreads) nan |= p_s[k] != p_s[k];
+    for (int k = tid; k < a.top; k += THREADS) nan |= p_s[k] != p_s[k];
     top = warp_max(top);
-    for (int k = tid; k < a.top; k += kThreads) total += exp2f((p_s[k] - finite_max(top)) * scale);
+    for (int k = tid; k < a.top; k += THREADS) total += exp2f((p_s[k] - finite_max(top)) * scale);
     total = warp_sum(total);
     bad = __any_sync(0xffffffffu, bad);
     if (lane == 0) {
@@ -221,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, kResident) distill_rows(const Distil
     if (!__syncthreads_or(any || nan)) {  // no teacher
         if (!BACKWARD && tid == 0 && rank == 0) a.row_loss[r] = 0.f;
         if (grad != nullptr)
-            for (int j = at.lo + tid; j < at.hi; j += kThreads) grad[j] = from_float<T>(0.f);
+            for (int j = at.lo + tid; j < at.hi; j += THREADS) grad[j] = from_float<T>(0.f);
         return;  // every CTA of the cluster does
     }
     {
@@ -230,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, kResident) distill_rows(const Distil
         total = warp_sum(lane < kWarps ? w.y * exp2f((w.x - finite_max(top)) * scale) : 0.f);
         bad = __any_sync(0xffffffffu, bad_s[lane % kWarps] != 0);
     }
-    for (int k = tid; k < a.top; k += kThreads) {
+    for (int k = tid; k < a.top; k += THREADS) {
         const int j = i_s[k] - at.lo;
         if (a.words == 0 || i_s[k] < at.lo || i_s[k] >= at.hi) continue;
         const unsigned bit = 1u << (j % 32);
@@ -247,14 +248,14 @@ __global__ void __launch_bounds__(kThreads, kResident) distill_rows(const Distil
             const float v[2] = {to_float(row[j]), -INFINITY};
             run.add<2>(v[0], v, scale, slack);
         };
-        for (int j = at.lo + tid; j < at.body; j += kThreads) one(j);
-        for (int j = at.tail() + tid; j < at.hi; j += kThreads) one(j);
+        for (int j = at.lo + tid; j < at.body; j += THREADS) one(j);
+        for (int j = at.tail() + tid; j < at.hi; j += THREADS) one(j);
         const T *body = row + at.body;
         int i = tid;
-        for (; i + 3 * kThreads < at.vecs; i += 4 * kThreads) {
+        for (; i + 3 * THREADS < at.vecs; i += 4 * THREADS) {
             RawVec<T, kVec> p[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) p[u].load(body + (i + u * kThreads) * kVec);
+            for (int u = 0; u < 4; ++u) p[u].load(body + (i + u * THREADS) * kVec);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 float v[kVec];
@@ -262,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, kResident) distill_rows(const Distil
                 run.add<kVec>(p[u].top(), v, scale, slack);
             }
         }
-        for (; i < at.vecs; i += kThreads) {
+        for (; i < at.vecs; i += THREADS) {
             RawVec<T, kVec> p;
             float v[kVec];
             p.load(body + i * kVec);
@@ -293,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, kResident) distill_rows(const Distil
     if (!BACKWARD && rank == 0) {
         const float log_total = log2f(total), log_sum = log2f(sum);
         float loss = 0.f;
-        for (int k = tid; k < a.top; k += kThreads) {
+        for (int k = tid; k < a.top; k += THREADS) {
             if (i_s[k] < 0) continue;
             const float lp = (p_s[k] - top) * scale - log_total, p = exp2f(lp);
             const float lq = (to_float(row[i_s[k]]) - m) * scale - log_sum;
@@ -323,23 +324,23 @@ __global__ void __launch_bounds__(kThreads, kResident) distill_rows(const Distil
             }
         };
         if ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(grad)) % 16 == 0) {
-            for (int j = at.lo + tid; j < at.body; j += kThreads) one(j);
-            for (int j = at.tail() + tid; j < at.hi; j += kThreads) one(j);
+            for (int j = at.lo + tid; j < at.body; j += THREADS) one(j);
+            for (int j = at.tail() + tid; j < at.hi; j += THREADS) one(j);
             const T *body = row + at.body;
             T *out = grad + at.body;
             int i = tid;
-            for (; i + 3 * kThreads < at.vecs; i += 4 * kThreads) {
+            for (; i + 3 * THREADS < at.vecs; i += 4 * THREADS) {
                 RawVec<T, kVec> p[4];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) p[u].load(body + (i + u * kThreads) * kVec);
+                for (int u = 0; u < 4; ++u) p[u].load(body + (i + u * THREADS) * kVec);
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     float v[kVec];
                     gradients(p[u], v);
-                    store_packed<T, kVec>(out + (i + u * kThreads) * kVec, v);
+                    store_packed<T, kVec>(out + (i + u * THREADS) * kVec, v);
                 }
             }
-            for (; i < at.vecs; i += kThreads) {
+            for (; i < at.vecs; i += THREADS) {
                 RawVec<T, kVec> p;
                 float v[kVec];
                 p.load(body + i * kVec);
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, kResident) distill_rows(const Distil
                 store_packed<T, kVec>(out + i * kVec, v);
             }
         } else {  // rows of logits and gradient fall differently on 16 bytes
-            for (int j = at.lo + tid; j < at.hi; j += kThreads) one(j);
+            for (int j = at.lo + tid; j < at.hi; j += THREADS) one(j);
         }
     }
     __syncthreads();
@@ -361,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, kResident) distill_rows(const Distil
     // the entries the teacher names: q - p, the p of an entry named twice added up by the first
     const float per = 1.f / total;
     const bool again = a.words == 0 || again_s != 0;
-    for (int k = tid; k < a.top; k += kThreads) {
+    for (int k = tid; k < a.top; k += THREADS) {
         const int j = i_s[k];
         if (j < at.lo || j >= at.hi) continue;
         float p = exp2f((p_s[k] - top) * scale) * per;
@@ -404,10 +405,17 @@ template <typename T> __global__ void __launch_bounds__(256) distill_scale(T *gr
         grad[i] = from_float<T>(to_float(grad[i]) * f);
 }
 
+template <typename T, int THREADS>
+cudaError_t launch_kernel(cudaLaunchConfig_t &config, const DistillArgs &a, bool backward) {
+    config.blockDim = dim3(THREADS);
+    return backward ? cudaLaunchKernelEx(&config, distill_rows<T, true, THREADS>, a)
+                    : cudaLaunchKernelEx(&config, distill_rows<T, false, THREADS>, a);
+}
 template <typename T> int launch_rows(DistillArgs a, bool backward, cudaStream_t st) {
     // Rows alone fill the SMs from 148 on; fewer are split down to 4,096 logits a CTA.  Long ones are split so
-    // that the second pass finds its logits in L2: 6 CTAs an SM of 80 KB are 71 MB.  (When chosen: 8,192 x 32,000 bf16 unsplit 215
-    // us, halved 297.  2,048 x 32,000 f32: halved 114, unsplit 133.  2,048 x 128,000 bf16: quarters, 248.)
+    // that the second pass finds its logits in L2: 6 CTAs an SM of 80 KB are 71 MB.  (When chosen: 8,192 x 32,000
+    // bf16 unsplit 215 us, halved 297.  2,048 x 32,000 f32: halved 114, unsplit 133.  2,048 x 128,000 bf16: quarters,
+    // 248.)
     int ranks = 1;
     while (ranks < kMaxCluster &&
            ((a.rows * ranks * 2 <= 296 && a.vocab / (ranks * 2) >= 4096) ||
@@ -417,7 +425,6 @@ template <typename T> int launch_rows(DistillArgs a, bool backward, cudaStream_t
     a.words = longest * static_cast<long>(sizeof(T)) <= 2 * kStretchBytes ? static_cast<int>((longest + 31) / 32) : 0;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(static_cast<unsigned>(a.rows * ranks));
-    config.blockDim = dim3(kThreads);
     config.dynamicSmemBytes = static_cast<size_t>(a.words) * sizeof(unsigned);
     config.stream = st;
     cudaLaunchAttribute attribute{};
@@ -425,9 +432,14 @@ template <typename T> int launch_rows(DistillArgs a, bool backward, cudaStream_t
     attribute.val.clusterDim.x = static_cast<unsigned>(ranks);
     attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
     config.attrs = &attribute;
-    config.numAttrs = 1;
-    const cudaError_t e = backward ? cudaLaunchKernelEx(&config, distill_rows<T, true>, a)
-                                   : cudaLaunchKernelEx(&config, distill_rows<T, false>, a);
+    config.numAttrs = ranks > 1 ? 1 : 0;  // a cluster of one costs: 65,536 x 256 bf16 289 us with it, 159 without
+    // Short rows are bound by a row's chain of round trips, so more of them at a time, by fewer threads each.  64, 128
+    // and 256 threads: 65,536 x 256 bf16 159, 244, 452 us; 32,768 x 4,096 bf16 159, 196, 318; 32,768 x 4,096 f32 249,
+    // 239, 321; 8,192 x 16,000 bf16 177, 118, 142; 8,192 x 32,000 bf16 (12 rows an SM are then more than L2) -, 258, 204.
+    const long bytes = static_cast<long>(a.vocab) * static_cast<long>(sizeof(T));
+    const cudaError_t e = ranks > 1 || bytes > 32768 ? launch_kernel<T, 256>(config, a, backward)
+                          : bytes > 8192             ? launch_kernel<T, 128>(config, a, backward)
+                                                     : launch_kernel<T, 64>(config, a, backward);
     if (e != cudaSuccess) return fail(BSSM_ERR_CUDA, "distillation: %s", cudaGetErrorString(e));
     return check_launch("distillation");
 }
@@ -437,6 +449,10 @@ int launch_rows(int dtype, const DistillArgs &a, bool backward, cudaStream_t st)
         case BSSM_BF16: return launch_rows<__nv_bfloat16>(a, backward, st);
         default: return launch_rows<__half>(a, backward, st);
     }
+}
+
+int *counts_of(int mean, long rows, int top, int *counts) {
+    return mean && (rows > kCountRows || rows * top > kCountEntries) ? counts : nullptr;
 }
 
 int check_distill(const char *what, int dtype, long rows, int vocab, long row_stride, int top, int teacher_dtype,
@@ -471,9 +487,9 @@ extern "C" int bssm_distillation(const void *logits, int dtype, long rows, int v
     DistillArgs a{};
     a.logits = logits; a.teacher = teacher; a.indices = indices; a.rows = rows; a.row_stride = row_stride;
     a.vocab = vocab; a.top = top; a.teacher_dtype = teacher_dtype; a.wide_indices = index_bytes == 8;
-    a.temperature = temperature; a.mean = mean; a.counts = counts; a.row_loss = row_loss;
+    a.temperature = temperature; a.mean = mean; a.counts = counts_of(mean, rows, top, counts); a.row_loss = row_loss;
     a.row_stats = reinterpret_cast<float2 *>(row_stats); a.grad = grad;
-    if (mean && rows * top > kCountHere) {
+    if (a.counts != nullptr) {
         distill_count<<<kCounters, 1024, 0, st>>>(a);
         if (int rc = check_launch("distillation")) return rc;
     }
@@ -501,7 +517,8 @@ extern "C" int bssm_distillation_backward(const void *logits, int dtype, long ro
     DistillArgs a{};
     a.logits = logits; a.teacher = teacher; a.indices = indices; a.rows = rows; a.row_stride = row_stride;
     a.vocab = vocab; a.top = top; a.teacher_dtype = teacher_dtype; a.wide_indices = index_bytes == 8;
-    a.temperature = temperature; a.mean = mean; a.counts = const_cast<int *>(counts);
+    a.temperature = temperature; a.mean = mean;
+    a.counts = counts_of(mean, rows, top, const_cast<int *>(counts));
     a.row_stats = reinterpret_cast<float2 *>(const_cast<float *>(row_stats));
     a.grad = grad; a.upstream = upstream; a.upstream_per_row = upstream_per_row;
     return launch_rows(dtype, a, true, static_cast<cudaStream_t>(stream));

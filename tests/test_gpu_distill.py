@@ -238,3 +238,26 @@ def test_refusals_on_the_gpu():
         distillation_loss(logits.double(), teacher, indices)
     with pytest.raises(ValueError, match="same device"):
         distillation_loss(logits, teacher, indices.cpu())
+
+
+# rows of up to 8 KB, of up to 32 KB and longer ones (64, 128 and 256 threads a row), around the lengths where the form
+# changes; 16 rows count those with a teacher themselves, 17 do not
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("rows,vocab,top", [(16, 2048, 20), (17, 2049, 20), (40, 4096, 100), (16, 4097, 1000),
+                                            (17, 8192, 5), (33, 8193, 64), (16, 16384, 256), (17, 16385, 257)])
+def test_row_lengths_where_the_form_changes(rows, vocab, top, dtype):
+    logits, teacher, indices = inputs(rows, vocab, top, dtype, 3 * rows + vocab)
+    indices[rows // 2] = -1
+    indices[0, top // 2] = indices[0, 0]  # named twice
+    for reduction in ("mean", "none"):
+        want, x64 = reference(logits, teacher, indices, 1.5, reduction)
+        x = logits.detach().requires_grad_()
+        loss = distillation_loss(x, teacher, indices, temperature=1.5, reduction=reduction)
+        assert float((loss.detach().double() - want.detach()).abs().max()) <= \
+            1e-5 * (float(want.detach().abs().max()) + 1.5 ** 2)
+        up = torch.ones_like(want)
+        got = torch.autograd.grad(loss, x, up.float(), retain_graph=True)[0]
+        ref = torch.autograd.grad(want, x64, up)[0]
+        assert rel(got, ref) <= TOL[dtype] and not got[rows // 2].any()
+        again = torch.autograd.grad(loss, x, up.float())[0]  # from the rows' statistics
+        assert rel(again, ref) <= TOL[dtype]
