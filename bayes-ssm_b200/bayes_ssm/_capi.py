@@ -81,7 +81,8 @@ _SIGNATURES = {
                            _vp], _i),
     "bssm_distillation_backward": ([_vp, _i, _l, _i, _l, _vp, _i, _vp, _i, _i, ctypes.c_float, _i, _vp, _vp, _vp, _i,
                                     _vp, _vp], _i),
-    "bssm_distillation_scale": ([_vp, _i, _l, _vp, _vp], _i),
+    "bssm_distillation_rescale": ([_vp, _i, _l, _i, _l, _vp, _i, _vp, _i, _i, ctypes.c_float, _i, _vp, _vp, _vp, _vp,
+                                   _vp], _i),
     "bssm_debug_wait_timeouts": ([], ctypes.c_uint),
     "bssm_stream_status": ([_vp], _i),
     "bssm_debug_wait_probe": ([_i, _vp], _i),

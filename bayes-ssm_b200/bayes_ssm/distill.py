@@ -84,22 +84,21 @@ class _Distillation(torch.autograd.Function):
         temperature, reduction = ctx.settings
         dev = logits.device
         upstream = upstream.float().contiguous()
-        # The gradient written by the forward is handed out once, times the
-        # upstream one; a second walk through a retained graph makes its own.
-        grad, ctx.grad = ctx.grad, None
-        if grad is not None:
-            _capi.launch(dev, "bssm_distillation_scale", grad.data_ptr(), _DTYPES[grad.dtype], grad.numel(),
-                         upstream.data_ptr())
-            return grad, None, None, None, None
         x, stride = _rows(logits, 1)
         top = teacher.shape[-1]
         rows = teacher.numel() // top
-        grad = _empty_like(logits)
         at = scratch.data_ptr()
-        _capi.launch(dev, "bssm_distillation_backward", x.data_ptr(), _DTYPES[x.dtype], rows, logits.shape[-1],
-                     stride, teacher.data_ptr(), _DTYPES[teacher.dtype], indices.data_ptr(), indices.element_size(),
-                     top, temperature, reduction == "mean", at, at + 12 * rows, upstream.data_ptr(),
-                     reduction == "none", grad.data_ptr())
+        flat = (x.data_ptr(), _DTYPES[x.dtype], rows, logits.shape[-1], stride, teacher.data_ptr(),
+                _DTYPES[teacher.dtype], indices.data_ptr(), indices.element_size(), top, temperature,
+                reduction == "mean", at, at + 12 * rows, upstream.data_ptr())
+        # The gradient written by the forward is handed out once, as it is where the upstream one is 1 and computed
+        # again where not (the factor comes before the rounding); a second walk through a retained graph makes its own.
+        grad, ctx.grad = ctx.grad, None
+        if grad is not None:
+            _capi.launch(dev, "bssm_distillation_rescale", *flat, grad.data_ptr())
+        else:
+            grad = _empty_like(logits)
+            _capi.launch(dev, "bssm_distillation_backward", *flat, reduction == "none", grad.data_ptr())
         return grad, None, None, None, None
 
 

@@ -31,6 +31,7 @@ namespace bssm {
 namespace {
 
 constexpr int kThreadsAnSM = 1536;  // 6 CTAs of 256 threads, 12 of 128 or 24 of 64
+constexpr int kRescaleThreadsAnSM = 1280;  // 48 registers: a loop over rows does not fit 40 (64: within 3 %)
 constexpr long kStretchBytes = 81920;  // longest stretch of a row that a CTA takes while clusters allow it
 constexpr int kMaxTop = 1024;
 constexpr int kCounters = 148;       // partial counts of the rows with a teacher
@@ -164,13 +165,13 @@ struct Running {
     }
 };
 
-// BACKWARD: the reference and sum are the forward's.
+// Row r by a CTA or, rank by rank, by its cluster.  BACKWARD: the reference and sum are the forward's.
 // 8,192 x 32,000 bf16, K 64, loss and gradient: 204 us for 1.05 GB (5.1 TB/s,
 // 0.80 of a copy's rate; the exp2 unit at 59 %); 2,048 x 32,000 f32, K 32: 112
 // us (4.7 TB/s); 4 x 50,001 bf16 in clusters of 8: 10 us.  Rows of a few hundred
 // logits are bound by their chain of round trips (65,536 x 256: 159 us, 2.4 ns a row).
 template <typename T, bool BACKWARD, int THREADS>
-__global__ void __launch_bounds__(THREADS, kThreadsAnSM / THREADS) distill_rows(const DistillArgs a) {
+__device__ __forceinline__ void distill_row(const DistillArgs &a, const long r) {
     constexpr int kVec = 16 / sizeof(T), kWarps = THREADS / 32;
     __shared__ float p_s[kMaxTop];
     __shared__ __align__(16) int i_s[kMaxTop + 4];
@@ -182,7 +183,6 @@ __global__ void __launch_bounds__(THREADS, kThreadsAnSM / THREADS) distill_rows(
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = static_cast<int>(cluster.block_rank()), ranks = static_cast<int>(cluster.num_blocks());
-    const long r = blockIdx.x / ranks;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const T *row = static_cast<const T *>(a.logits) + r * a.row_stride;
     T *grad = a.grad == nullptr ? nullptr : static_cast<T *>(a.grad) + r * a.vocab;
@@ -379,6 +379,25 @@ __global__ void __launch_bounds__(THREADS, kThreadsAnSM / THREADS) distill_rows(
         grad[j] = from_float<T>(weight * (exp2_unit((to_float(row[j]) - m) * scale) * inverse - p));
     }
 }
+template <typename T, bool BACKWARD, int THREADS>
+__global__ void __launch_bounds__(THREADS, kThreadsAnSM / THREADS) distill_rows(const DistillArgs a) {
+    distill_row<T, BACKWARD, THREADS>(a, blockIdx.x / cooperative_groups::this_cluster().num_blocks());
+}
+// The gradient that the forward wrote, computed again for an upstream factor,
+// which has to come before the rounding: a loss scale saves gradients that 16
+// bits cannot hold.  Nothing at all where the factor is 1 (the loss was the end
+// of the graph); one wave of CTAs, so that this is then over in 1 to 3 us.
+// 8,192 x 32,000 bf16: 211 us (one read and one write of the logits' bytes, 5.0
+// TB/s); 2,048 x 32,000 f32: 107; 65,536 x 256 bf16, by the rows' chains: 128.
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, kRescaleThreadsAnSM / THREADS) distill_rescale(const DistillArgs a) {
+    if (*a.upstream == 1.f) return;
+    const unsigned ranks = cooperative_groups::this_cluster().num_blocks();
+    for (unsigned r = blockIdx.x / ranks; r < a.rows; r += gridDim.x / ranks) {
+        distill_row<T, true, THREADS>(a, r);
+        __syncthreads();  // the row's entries have been read
+    }
+}
 
 // The rows' losses added in a fixed order, and divided by the rows counted.
 constexpr int kTotalThreads = 1024;
@@ -397,21 +416,18 @@ __global__ void __launch_bounds__(kTotalThreads) distill_total(const DistillArgs
     if (threadIdx.x == 0) *loss = v / static_cast<float>(max(1, n));
 }
 
-// grad *= *factor, nothing at all where it is 1 (the loss was the end of the graph).
-template <typename T> __global__ void __launch_bounds__(256) distill_scale(T *grad, long n, const float *factor) {
-    const float f = *factor;
-    if (f == 1.f) return;
-    for (long i = static_cast<long>(blockIdx.x) * 256 + threadIdx.x; i < n; i += 256L * gridDim.x)
-        grad[i] = from_float<T>(to_float(grad[i]) * f);
-}
+enum RowsKind { kForward, kBackward, kRescale };
 
 template <typename T, int THREADS>
-cudaError_t launch_kernel(cudaLaunchConfig_t &config, const DistillArgs &a, bool backward) {
+cudaError_t launch_kernel(cudaLaunchConfig_t &config, unsigned ranks, const DistillArgs &a, RowsKind kind) {
     config.blockDim = dim3(THREADS);
-    return backward ? cudaLaunchKernelEx(&config, distill_rows<T, true, THREADS>, a)
-                    : cudaLaunchKernelEx(&config, distill_rows<T, false, THREADS>, a);
+    if (kind == kForward) return cudaLaunchKernelEx(&config, distill_rows<T, false, THREADS>, a);
+    if (kind == kBackward) return cudaLaunchKernelEx(&config, distill_rows<T, true, THREADS>, a);
+    const unsigned wave = 148u * (kRescaleThreadsAnSM / THREADS) / ranks * ranks;
+    if (config.gridDim.x > wave) config.gridDim.x = wave;
+    return cudaLaunchKernelEx(&config, distill_rescale<T, THREADS>, a);
 }
-template <typename T> int launch_rows(DistillArgs a, bool backward, cudaStream_t st) {
+template <typename T> int launch_rows(DistillArgs a, RowsKind kind, cudaStream_t st) {
     // Rows alone fill the SMs from 148 on; fewer are split down to 4,096 logits a CTA.  Long ones are split so
     // that the second pass finds its logits in L2: 6 CTAs an SM of 80 KB are 71 MB.  (When chosen: 8,192 x 32,000
     // bf16 unsplit 215 us, halved 297.  2,048 x 32,000 f32: halved 114, unsplit 133.  2,048 x 128,000 bf16: quarters,
@@ -437,17 +453,18 @@ template <typename T> int launch_rows(DistillArgs a, bool backward, cudaStream_t
     // and 256 threads: 65,536 x 256 bf16 159, 244, 452 us; 32,768 x 4,096 bf16 159, 196, 318; 32,768 x 4,096 f32 249,
     // 239, 321; 8,192 x 16,000 bf16 177, 118, 142; 8,192 x 32,000 bf16 (12 rows an SM are then more than L2) -, 258, 204.
     const long bytes = static_cast<long>(a.vocab) * static_cast<long>(sizeof(T));
-    const cudaError_t e = ranks > 1 || bytes > 32768 ? launch_kernel<T, 256>(config, a, backward)
-                          : bytes > 8192             ? launch_kernel<T, 128>(config, a, backward)
-                                                     : launch_kernel<T, 64>(config, a, backward);
+    const unsigned split = static_cast<unsigned>(ranks);
+    const cudaError_t e = ranks > 1 || bytes > 32768 ? launch_kernel<T, 256>(config, split, a, kind)
+                          : bytes > 8192             ? launch_kernel<T, 128>(config, split, a, kind)
+                                                     : launch_kernel<T, 64>(config, split, a, kind);
     if (e != cudaSuccess) return fail(BSSM_ERR_CUDA, "distillation: %s", cudaGetErrorString(e));
     return check_launch("distillation");
 }
-int launch_rows(int dtype, const DistillArgs &a, bool backward, cudaStream_t st) {
+int launch_rows(int dtype, const DistillArgs &a, RowsKind kind, cudaStream_t st) {
     switch (dtype) {
-        case BSSM_F32: return launch_rows<float>(a, backward, st);
-        case BSSM_BF16: return launch_rows<__nv_bfloat16>(a, backward, st);
-        default: return launch_rows<__half>(a, backward, st);
+        case BSSM_F32: return launch_rows<float>(a, kind, st);
+        case BSSM_BF16: return launch_rows<__nv_bfloat16>(a, kind, st);
+        default: return launch_rows<__half>(a, kind, st);
     }
 }
 
@@ -494,25 +511,24 @@ extern "C" int bssm_distillation(const void *logits, int dtype, long rows, int v
         if (int rc = check_launch("distillation")) return rc;
     }
     if (rows > 0)
-        if (int rc = launch_rows(dtype, a, false, st)) return rc;
+        if (int rc = launch_rows(dtype, a, kForward, st)) return rc;
     if (loss == nullptr) return BSSM_OK;
     distill_total<<<1, kTotalThreads, 0, st>>>(a, loss);
     return check_launch("distillation");
 }
 
-extern "C" int bssm_distillation_backward(const void *logits, int dtype, long rows, int vocab, long row_stride,
-                                          const void *teacher, int teacher_dtype, const void *indices, int index_bytes,
-                                          int top, float temperature, int mean, const float *row_stats,
-                                          const int *counts, const float *upstream, int upstream_per_row, void *grad,
-                                          void *stream) {
-    using namespace bssm;
-    if (int rc = check_distill("distillation_backward", dtype, rows, vocab, row_stride, top, teacher_dtype, index_bytes,
-                               temperature))
+namespace bssm {
+namespace {
+int launch_backward(const char *what, const void *logits, int dtype, long rows, int vocab, long row_stride,
+                    const void *teacher, int teacher_dtype, const void *indices, int index_bytes, int top,
+                    float temperature, int mean, const float *row_stats, const int *counts, const float *upstream,
+                    int upstream_per_row, RowsKind kind, void *grad, void *stream) {
+    if (int rc = check_distill(what, dtype, rows, vocab, row_stride, top, teacher_dtype, index_bytes, temperature))
         return rc;
     if ((rows > 0 && (logits == nullptr || teacher == nullptr || indices == nullptr || row_stats == nullptr ||
                       grad == nullptr)) ||
-        (mean && counts == nullptr))
-        return fail(BSSM_ERR_INVALID, "distillation_backward: null pointer");
+        (mean && counts == nullptr) || (kind == kRescale && upstream == nullptr))
+        return fail(BSSM_ERR_INVALID, "%s: null pointer", what);
     if (rows == 0) return BSSM_OK;
     DistillArgs a{};
     a.logits = logits; a.teacher = teacher; a.indices = indices; a.rows = rows; a.row_stride = row_stride;
@@ -521,20 +537,26 @@ extern "C" int bssm_distillation_backward(const void *logits, int dtype, long ro
     a.counts = counts_of(mean, rows, top, const_cast<int *>(counts));
     a.row_stats = reinterpret_cast<float2 *>(const_cast<float *>(row_stats));
     a.grad = grad; a.upstream = upstream; a.upstream_per_row = upstream_per_row;
-    return launch_rows(dtype, a, true, static_cast<cudaStream_t>(stream));
+    return launch_rows(dtype, a, kind, static_cast<cudaStream_t>(stream));
+}
+}  // namespace
+}  // namespace bssm
+
+extern "C" int bssm_distillation_backward(const void *logits, int dtype, long rows, int vocab, long row_stride,
+                                          const void *teacher, int teacher_dtype, const void *indices, int index_bytes,
+                                          int top, float temperature, int mean, const float *row_stats,
+                                          const int *counts, const float *upstream, int upstream_per_row, void *grad,
+                                          void *stream) {
+    return bssm::launch_backward("distillation_backward", logits, dtype, rows, vocab, row_stride, teacher,
+                                 teacher_dtype, indices, index_bytes, top, temperature, mean, row_stats, counts,
+                                 upstream, upstream_per_row, bssm::kBackward, grad, stream);
 }
 
-extern "C" int bssm_distillation_scale(void *grad, int dtype, long n, const float *factor, void *stream) {
-    using namespace bssm;
-    if (!io_dtype_known(dtype)) return fail(BSSM_ERR_UNSUPPORTED, "distillation_scale: unknown dtype");
-    if (n < 0 || factor == nullptr || (n > 0 && grad == nullptr))
-        return fail(BSSM_ERR_INVALID, "distillation_scale: bad arguments");
-    if (n == 0) return BSSM_OK;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const long blocks = (n + 2047) / 2048;
-    const unsigned grid = static_cast<unsigned>(blocks < 1184 ? blocks : 1184);
-    if (dtype == BSSM_F32) distill_scale<<<grid, 256, 0, st>>>(static_cast<float *>(grad), n, factor);
-    else if (dtype == BSSM_BF16) distill_scale<<<grid, 256, 0, st>>>(static_cast<__nv_bfloat16 *>(grad), n, factor);
-    else distill_scale<<<grid, 256, 0, st>>>(static_cast<__half *>(grad), n, factor);
-    return check_launch("distillation_scale");
+extern "C" int bssm_distillation_rescale(const void *logits, int dtype, long rows, int vocab, long row_stride,
+                                         const void *teacher, int teacher_dtype, const void *indices, int index_bytes,
+                                         int top, float temperature, int mean, const float *row_stats,
+                                         const int *counts, const float *upstream, void *grad, void *stream) {
+    return bssm::launch_backward("distillation_rescale", logits, dtype, rows, vocab, row_stride, teacher,
+                                 teacher_dtype, indices, index_bytes, top, temperature, mean, row_stats, counts,
+                                 upstream, 0, bssm::kRescale, grad, stream);
 }

@@ -513,7 +513,10 @@ int bssm_selective_step(const void *values, long value_stride, const void *steps
  * ints) is scratch that the backward reads again.  grad (may be null)
  * [rows][vocab] receives the gradient of that loss; the backward writes it
  * times *upstream, or times upstream[row].
- * bssm_distillation_scale multiplies n values by the device float *factor.
+ * bssm_distillation_rescale makes the grad that bssm_distillation wrote that of
+ * the loss times *upstream: it computes it again, so that the factor comes
+ * before the one rounding (a loss scale would otherwise come after what it is
+ * to save was lost), and leaves it as it is where *upstream is 1.
  */
 int bssm_distillation_counters(void);
 int bssm_distillation(const void *logits, int dtype, long rows, int vocab, long row_stride, const void *teacher,
@@ -523,7 +526,10 @@ int bssm_distillation_backward(const void *logits, int dtype, long rows, int voc
                                const void *teacher, int teacher_dtype, const void *indices, int index_bytes, int top,
                                float temperature, int mean, const float *row_stats, const int *counts,
                                const float *upstream, int upstream_per_row, void *grad, void *stream);
-int bssm_distillation_scale(void *grad, int dtype, long n, const float *factor, void *stream);
+int bssm_distillation_rescale(const void *logits, int dtype, long rows, int vocab, long row_stride,
+                              const void *teacher, int teacher_dtype, const void *indices, int index_bytes, int top,
+                              float temperature, int mean, const float *row_stats, const int *counts,
+                              const float *upstream, void *grad, void *stream);
 
 /*
  * Device status (no counterpart in the reference: its kernels have no waits).

@@ -261,3 +261,48 @@ def test_row_lengths_where_the_form_changes(rows, vocab, top, dtype):
         assert rel(got, ref) <= TOL[dtype] and not got[rows // 2].any()
         again = torch.autograd.grad(loss, x, up.float())[0]  # from the rows' statistics
         assert rel(again, ref) <= TOL[dtype]
+
+
+def grad64(logits, teacher, indices, temperature):
+    """The gradient of every row's loss in 64 bits (every row has a teacher, no entry is empty)."""
+    q = torch.softmax(logits.double() / temperature, -1)
+    p = torch.softmax(teacher.double() / temperature, -1)
+    return temperature * q.scatter_add(1, indices, -p)
+
+
+# an entry of the gradient differs from the 64-bit one's rounding only where that lies within its float32 error, 2.6e-6
+# of itself outside the teacher's entries, of a boundary between two numbers of the type: these are at least 2^-8
+# (bfloat16) and 2^-11 (float16) of it apart, so 2 * 2.6e-6 * 2^8 = 0.14 % and 1.1 % of the entries
+@pytest.mark.parametrize("dtype,differ", [(torch.bfloat16, 1.4e-3), (torch.float16, 1.1e-2)])
+@pytest.mark.parametrize("vocab", (2001, 2048))
+@pytest.mark.parametrize("reduction,factor", [("mean", 65536.0), ("sum", 0.3), ("mean", -5000.0)])
+def test_upstream_factor_before_the_one_rounding(reduction, factor, vocab, dtype, differ):
+    """A loss scale reaches the gradient before it is rounded: unscaled, most of this one is below float16's least."""
+    rows = 4096
+    logits, teacher, indices = inputs(rows, vocab, 16, dtype, 21)
+    up = torch.tensor(factor, device="cuda")
+    ref = grad64(logits, teacher, indices, 2.0) * up.double() / (rows if reduction == "mean" else 1)
+    x = logits.requires_grad_()
+    loss = distillation_loss(x, teacher, indices, temperature=2.0, reduction=reduction)
+    got = torch.autograd.grad(loss, x, up, retain_graph=True)[0]
+    others = torch.ones_like(logits, dtype=torch.bool).scatter_(1, indices, False)
+    assert float((got != ref.to(dtype))[others].double().mean()) <= differ
+    assert rel(got, ref) <= TOL[dtype]
+    assert torch.equal(torch.autograd.grad(loss, x, up)[0], got)  # a second walk
+
+
+def test_upstream_factor_of_every_form():
+    """The factor at few rows (split over clusters), many, rows without a teacher, and factors that are not finite."""
+    for rows, vocab, top in ((2, 50001, 16), (3000, 300, 4), (20, 20000, 9), (5, 1, 1)):
+        logits, teacher, indices = inputs(rows, vocab, top, torch.float32, 22)
+        ref = grad64(logits, teacher, indices, 1.0) * 7.0
+        indices[1] = -1
+        x = logits.requires_grad_()
+        loss = distillation_loss(x, teacher, indices, reduction="sum")
+        got = torch.autograd.grad(loss, x, torch.tensor(7.0, device="cuda"), retain_graph=True)[0]
+        ref[1] = 0
+        if vocab > 1:
+            assert rel(got, ref) <= 1e-5
+        assert not got[1].any()
+        nan = torch.autograd.grad(loss, x, torch.tensor(math.nan, device="cuda"))[0]
+        assert torch.isnan(nan[0]).all() and not nan[1].any()
