@@ -37,12 +37,12 @@ def distillation_loss_torch(logits: Tensor, teacher_logits: Tensor, teacher_indi
     p = torch.where(live, torch.exp(log_p), 0.0)
     bad = (live & (teacher_indices >= logits.shape[-1])).any(-1)
     index = teacher_indices.long().clamp(0, logits.shape[-1] - 1)
-    s = torch.where((counted & ~bad)[..., None], logits.to(wide), 0.0)
+    # NaN by a factor, so that the gradient of a row with an entry past the vocabulary is NaN too
+    s = torch.where(counted[..., None], logits.to(wide), 0.0) * torch.where(bad, math.nan, 1.0).to(wide)[..., None]
     log_q = torch.gather(torch.log_softmax(s / temperature, -1), -1, index)
     # an entry of no weight adds nothing, whatever its logarithms
     term = torch.where(p != 0, p * (log_p - torch.where(p != 0, log_q, 0.0)), 0.0)
     rows = torch.where(counted, term.sum(-1) * temperature * temperature, 0.0)
-    rows = torch.where(bad, math.nan, rows)
     if reduction == "none":
         return rows
     total = rows.sum()

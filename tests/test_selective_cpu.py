@@ -237,3 +237,17 @@ def test_model_trains_from_a_teacher_and_generates():
     assert torch.equal(model(again)[0, 2:].argmax(-1), out[0])
     with pytest.raises(ValueError, match="at least one token"):
         model.prefill(tokens[:, :0])
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.float64))
+def test_an_entry_past_the_vocabulary_makes_the_gradient_nan(dtype):
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(4, 7, generator=g, dtype=dtype).requires_grad_()
+    teacher = torch.randn(4, 3, generator=g, dtype=dtype)
+    indices = torch.tensor([[0, 7, 2], [1, 2, 3], [-1, -1, -1], [6, 5, -1]])
+    for reduction in ("mean", "sum", "none"):
+        loss = distillation_loss(x, teacher, indices, reduction=reduction)
+        grad = torch.autograd.grad(loss.sum(), x)[0]
+        assert torch.isnan(loss).any() and torch.isnan(grad[0]).all(), reduction
+        assert torch.isfinite(grad[1:]).all() and not grad[2].any() and grad[1].any(), reduction
+    assert torch.isfinite(loss[1:]).all() and torch.isnan(loss[0])
