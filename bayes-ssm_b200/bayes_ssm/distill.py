@@ -110,11 +110,11 @@ def distillation_loss(logits: Tensor, teacher_logits: Tensor, teacher_indices: T
     teacher's logits at vocabulary entries ``teacher_indices [..., K]`` (int32
     or int64).  An entry with a negative index or a logit of ``-inf`` is empty;
     a row of empty entries (a prompt's, or padding) has loss and gradient zero
-    and does not count in a mean.  An index at or past V makes the row's loss
-    and gradient NaN.  ``reduction`` is ``"mean"`` (over the rows that count;
-    zero if none does), ``"sum"`` or ``"none"`` (``[...]``).  The loss is
-    float32; gradients flow to ``logits`` only.  CUDA takes up to 1,024 teacher
-    logits a row.
+    and does not count in a mean.  An index at or past V, or a teacher's logit
+    of NaN or ``+inf``, makes the row's loss and gradient NaN.  ``reduction``
+    is ``"mean"`` (over the rows that count; zero if none does), ``"sum"`` or
+    ``"none"`` (``[...]``).  The loss is float32; gradients flow to ``logits``
+    only.  CUDA takes up to 1,024 teacher logits a row.
     """
     if logits.ndim < 1 or teacher_logits.ndim != logits.ndim or teacher_logits.shape[:-1] != logits.shape[:-1]:
         raise ValueError("teacher_logits must be [..., K] with the logits' leading dimensions")

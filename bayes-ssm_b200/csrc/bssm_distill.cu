@@ -8,8 +8,9 @@
 //   ds_j = tau (q_j - sum_k [i_k = j] p_k) * upstream
 //
 // A row whose entries are all empty has no teacher: loss and gradient are
-// zero, and a mean does not count it.  An entry at or past V makes the row's
-// loss and gradient NaN (nothing is read or written out of range).
+// zero, and a mean does not count it.  An entry at or past V, or a teacher's
+// logit of NaN or +inf, makes the row's loss and gradient NaN (nothing is read
+// or written out of range).
 //
 // The traffic of the logits bounds it: read once, and the gradient written
 // once.  A CTA takes a row (where rows are few, a cluster of CTAs takes one,
@@ -288,8 +289,8 @@ __device__ __forceinline__ void distill_row(const DistillArgs &a, const long r) 
         }
         if (a.row_stats != nullptr && tid == 0 && rank == 0) a.row_stats[r] = stat;
     }
-    // a row of -inf alone has no distribution: m is -inf and what follows is NaN
-    const float m = stat.x, sum = stat.y, poison = bad ? NAN : 0.f, inverse = 1.f / sum + poison;
+    // a row of -inf alone has no distribution: m is -inf and what follows is NaN; so has a teacher's with a NaN or +inf
+    const float m = stat.x, sum = stat.y, poison = bad || total != total ? NAN : 0.f, inverse = 1.f / sum + poison;
 
     if (!BACKWARD && rank == 0) {
         const float log_total = log2f(total), log_sum = log2f(sum);

@@ -504,9 +504,10 @@ int bssm_selective_step(const void *values, long value_stride, const void *steps
  * 1,024) logits and q that of logits / temperature over `vocab`:
  * row_loss = temperature^2 sum_k p_k (log p_k - log q_{i_k}).  An index below
  * zero or a teacher logit of -inf is an empty entry; a row of empty entries
- * has loss and gradient zero; an index at or past vocab makes the row's loss
- * and gradient NaN.  logits rows are row_stride elements apart; teacher and
- * indices (index_bytes 4 or 8) are [rows][top].
+ * has loss and gradient zero; an index at or past vocab, or a teacher logit of
+ * NaN or +inf, makes the row's loss and gradient NaN.  logits rows are
+ * row_stride elements apart; teacher and indices (index_bytes 4 or 8) are
+ * [rows][top].
  * row_stats (two floats a row) is what the backward needs.  loss (may be
  * null) receives the sum of row_loss, divided, with mean != 0, by the number
  * of rows that have a teacher; for a mean, counts (bssm_distillation_counters()

@@ -306,3 +306,18 @@ def test_upstream_factor_of_every_form():
         assert not got[1].any()
         nan = torch.autograd.grad(loss, x, torch.tensor(math.nan, device="cuda"))[0]
         assert torch.isnan(nan[0]).all() and not nan[1].any()
+
+
+@pytest.mark.parametrize("value", (math.nan, math.inf))
+@pytest.mark.parametrize("rows,vocab", [(3, 500), (2, 50001)])
+def test_teacher_without_a_distribution(rows, vocab, value):
+    """A teacher's NaN or +inf leaves no softmax: the row's loss and whole gradient are NaN, as in PyTorch operations."""
+    logits, teacher, indices = inputs(rows, vocab, 4, torch.float32, 23)
+    teacher[1, 2] = value
+    x = logits.requires_grad_()
+    for form in (distillation_loss, distillation_loss_torch):
+        loss = form(x, teacher, indices, reduction="sum")
+        first = torch.autograd.grad(loss, x, retain_graph=True)[0]
+        second = torch.autograd.grad(loss, x)[0]
+        for grad in (first, second):
+            assert torch.isnan(grad[1]).all() and torch.isfinite(grad[0]).all() and torch.isfinite(grad[2:]).all()
