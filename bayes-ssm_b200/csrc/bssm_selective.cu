@@ -29,6 +29,7 @@
 // backward, beside the other float32 instructions of the step.
 #include <cuda_runtime.h>
 
+#include <cfloat>
 #include <cstdint>
 #include <type_traits>
 
@@ -197,6 +198,19 @@ __device__ __forceinline__ void store_states(float *p, int n0, int m, int states
     if (n0 + (1 ^ m) < states) p[1 ^ m] = v.y;
 }
 
+// A rate in powers of two.  One of -inf (a state that keeps nothing) becomes the
+// lowest number, so that a step of zero keeps the state whatever its rate: as
+// 0 * inf, the tokens that fill a tile up and the chunks past a short sequence's
+// end would make it NaN.
+__device__ __forceinline__ float in_powers_of_two(float rate) {
+    rate *= kLog2e;
+    return rate == -INFINITY ? -FLT_MAX : rate;
+}
+__device__ __forceinline__ float2 load_rates(const float *p, int n0, int m, int states) {
+    const float2 rate = load_states(p, n0, m, states);
+    return make_float2(in_powers_of_two(rate.x), in_powers_of_two(rate.y));
+}
+
 // The state that enters a chunk (BACKWARD: the adjoint, which enters at its
 // end).  A few chunks before (after) it are chained here, from what scan_local
 // found for each; more have been joined by scan_join.
@@ -334,7 +348,7 @@ template <typename T, int LPC> __global__ void __launch_bounds__(kThreads, 3) sc
     const int sub = lane / G::kPerWarp, c = tid / 32 * G::kPerWarp + lane % G::kPerWarp, n0 = 2 * sub;
     const bool live = c < p.width && n0 < a.states;
     const long row = static_cast<long>(a.channels) * a.states, at = static_cast<long>(p.c0 + c) * a.states + n0;
-    const float2 rate = mul2(load_states(live ? a.rates + at : nullptr, n0, 0, a.states), both(kLog2e));
+    const float2 rate = load_rates(live ? a.rates + at : nullptr, n0, 0, a.states);
     float2 h = entering<false>(a, p.s, chunk, p.c0 + c, at, n0, 0, live, rate);
 
     const long row0 = p.first + p.begin;
@@ -467,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 3) scan_local(const ScanArgs a) {
     const int sub = lane / G::kPerWarp, c = tid / 32 * G::kPerWarp + lane % G::kPerWarp, n0 = 2 * sub;
     const bool live = c < p.width && n0 < a.states;
     const long row = static_cast<long>(a.channels) * a.states, at = static_cast<long>(p.c0 + c) * a.states + n0;
-    const float2 rate = mul2(load_states(live ? a.rates + at : nullptr, n0, 0, a.states), both(kLog2e));
+    const float2 rate = load_rates(live ? a.rates + at : nullptr, n0, 0, a.states);
     float2 h = both(0.f);
     float span = 0.f;
 
@@ -567,7 +581,7 @@ template <bool BACKWARD> __global__ void __launch_bounds__(kThreads) scan_join(c
     const long i = static_cast<long>(blockIdx.x) * kThreads + threadIdx.x;
     if (i >= a.seq.count * row) return;
     const long s = i / row, at = i % row, c = at / a.states;
-    const float rate = a.rates[at] * kLog2e;
+    const float rate = in_powers_of_two(a.rates[at]);
     const float *start = BACKWARD ? a.grad_state1 : a.state0;
     float h = start != nullptr ? start[i] : 0.f;
 #pragma unroll 4
@@ -630,7 +644,7 @@ scan_backward(const ScanArgs a) {
     const int part_at = (keys_here ? G::kStates : 0) + n0 + m;
     const bool live = c < p.width && n0 < a.states;
     const long row = static_cast<long>(a.channels) * a.states, at = static_cast<long>(p.c0 + c) * a.states + n0;
-    const float2 rate = mul2(load_states(live ? a.rates + at : nullptr, n0, m, a.states), both(kLog2e));
+    const float2 rate = load_rates(live ? a.rates + at : nullptr, n0, m, a.states);
     float2 grate = both(0.f);
     float2 g = entering<true>(a, p.s, chunk, p.c0 + c, at, n0, m, live, rate);
     float gskip = 0.f, gbias = 0.f;
@@ -933,7 +947,7 @@ __global__ void __launch_bounds__(kThreads, 4) scan_step(const ScanArgs a, float
     const bool wide_k = aligned(a.keys, a.key_stride), wide_q = aligned(a.queries, a.query_stride);
     float rate[VEC], bias = 0.f, skip = 0.f;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) rate[j] = j < n ? a.rates[at + j] * kLog2e : 0.f;
+    for (int j = 0; j < VEC; ++j) rate[j] = j < n ? in_powers_of_two(a.rates[at + j]) : 0.f;
     if (live && a.step_bias != nullptr) bias = a.step_bias[c];
     if (live && a.skip != nullptr) skip = a.skip[c];
     long s = blockIdx.y;

@@ -427,3 +427,27 @@ def test_refusals_on_the_gpu():
         causal_conv(x, w, b, sequences=None, initial_state=s.cpu())
     with pytest.raises(ValueError, match="same device"):
         causal_conv(x[0], w, b, sequences=PackedSequences([5], device="cpu"))
+
+
+@pytest.mark.parametrize("shape,c", [((2, 37), 40), ((1, 5), 3), ((1, 64), 16), ([3300, 0, 130, 1700, 1], 24),
+                                     ([700, 3, 90], 24)])
+def test_rates_of_minus_infinity(shape, c):
+    """A state that keeps nothing from token to token, whatever the lengths: the tokens that fill a tile up have a step
+    of zero, and so do the chunks past a short sequence's end."""
+    i, lengths = scan_inputs(shape, c, 16, 1, torch.float32, 45)
+    i["rates"][::2, 1::3] = -torch.inf
+    i["rates"][1, 4] = torch.finfo(torch.float32).min
+    seqs = None if lengths is None else PackedSequences(lengths, device="cuda")
+    names = ("values", "keys", "queries", "skip", "gate")  # the others' gradients are products of infinity and zero
+    r = {n: v.double().requires_grad_(n in names) for n, v in i.items()}
+    k = {n: v.clone().requires_grad_(n in names) for n, v in i.items()}
+    want, want_final = call_plain(r, True, lengths)
+    y, final = call(k, True, seqs)
+    close(y, want, 2e-5, "read")
+    close(final, want_final, 2e-5, "state")
+    g = gen(46)
+    gy, gf = rand(g, *y.shape), rand(g, *final.shape)
+    got = torch.autograd.grad((y, final), [k[n] for n in names], (gy, gf))
+    ref = torch.autograd.grad((want, want_final), [r[n] for n in names], (gy.double(), gf.double()))
+    for name, a, b in zip(names, got, ref):
+        close(a, b, 2e-5, f"grad {name}")
