@@ -211,6 +211,13 @@ __device__ __forceinline__ float2 load_rates(const float *p, int n0, int m, int 
     return make_float2(in_powers_of_two(rate.x), in_powers_of_two(rate.y));
 }
 
+// The state after a chunk that h entered, exp(A D) h + local.  One of zero adds
+// nothing, also where exp(A D) is past float32 (a positive rate; token by token
+// it would never have been formed).
+__device__ __forceinline__ float through_chunk(float exponent, float h, float local) {
+    return h == 0.f ? local : fmaf(exp2f(exponent), h, local);
+}
+
 // The state that enters a chunk (BACKWARD: the adjoint, which enters at its
 // end).  A few chunks before (after) it are chained here, from what scan_local
 // found for each; more have been joined by scan_join.
@@ -228,7 +235,7 @@ __device__ __forceinline__ float2 entering(const ScanArgs &a, long s, int chunk,
         const long entry = s * a.chunks + k;
         const float span = live ? a.span[entry * a.channels + c] : 0.f;
         const float2 local = load_states(live ? a.carry + entry * row + at : nullptr, n0, m, a.states);
-        h = fma2(make_float2(exp2f(span * rate.x), exp2f(span * rate.y)), h, local);
+        h = make_float2(through_chunk(span * rate.x, h.x, local.x), through_chunk(span * rate.y, h.y, local.y));
     }
     return h;
 }
@@ -587,7 +594,7 @@ template <bool BACKWARD> __global__ void __launch_bounds__(kThreads) scan_join(c
 #pragma unroll 4
     for (int k = 0; k + 1 < a.chunks; ++k) {
         const long entry = s * a.chunks + (BACKWARD ? a.chunks - 1 - k : k);
-        h = fmaf(exp2f(a.span[entry * a.channels + c] * rate), h, a.carry[entry * row + at]);
+        h = through_chunk(a.span[entry * a.channels + c] * rate, h, a.carry[entry * row + at]);
         a.carry[entry * row + at] = h;
     }
 }

@@ -451,3 +451,26 @@ def test_rates_of_minus_infinity(shape, c):
     ref = torch.autograd.grad((want, want_final), [r[n] for n in names], (gy.double(), gf.double()))
     for name, a, b in zip(names, got, ref):
         close(a, b, 2e-5, f"grad {name}")
+
+
+@pytest.mark.parametrize("shape,n", [((1, 3400), 16), ((2, 700), 6)])
+def test_growing_states_that_are_still_zero(shape, n):
+    """Positive rates: a state (or an adjoint) of zero stays zero over a chunk whose growth float32 cannot hold.  The
+    values begin 20 tokens before the end (the reads' gradients end 20 tokens after the start), which grow as exp(40)."""
+    i, _ = scan_inputs(shape, 24, n, 1, torch.float32, 47)
+    i["rates"] = torch.full_like(i["rates"], 2.0)
+    i["steps"] = torch.full_like(i["steps"], 1.0)
+    i["state"] = i["step_bias"] = None
+    late = dict(i, values=i["values"].clone())
+    late["values"][:, :-20] = 0
+    want, want_final = call_plain({k: None if v is None else v.double() for k, v in late.items()}, False, None)
+    y, final = call(late, False, None)
+    close(y, want, 2e-5, "read")
+    close(final, want_final, 2e-5, "state")
+    early = dict(i, values=torch.zeros_like(i["values"]))
+    r = dict(zip(NAMES, leaves64(*(early[k] for k in NAMES))))
+    k = dict(zip(NAMES, leaves(*(early[k] for k in NAMES))))
+    gy = rand(gen(48), *y.shape)
+    gy[:, 20:] = 0
+    want = torch.autograd.grad(call_plain(r, False, None)[0], r["values"], gy.double())[0]
+    close(torch.autograd.grad(call(k, False, None)[0], k["values"], gy)[0], want, 2e-5, "grad values")
