@@ -19,7 +19,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _capi
-from .selective import _DTYPES, _empty_like, _gradients_wanted, _rows
+from .selective import _DTYPES, _carries_tangent, _empty_like, _gradients_wanted, _rows
 
 MAX_TOP = 1024
 
@@ -142,7 +142,7 @@ def distillation_loss(logits: Tensor, teacher_logits: Tensor, teacher_indices: T
         raise NotImplementedError(f"distillation_loss on CUDA needs at most {MAX_TOP} teacher logits a row "
                                   f"(got {teacher_logits.shape[-1]}); use distillation_loss_torch")
     teacher, indices = teacher_logits.detach().contiguous(), teacher_indices.contiguous()
-    if _gradients_wanted(logits):
+    if _gradients_wanted(logits) or _carries_tangent(logits):
         return _Distillation.apply(logits, teacher, indices, float(temperature), reduction)
     return _forward(logits, teacher, indices, float(temperature), reduction, False)[0]
 

@@ -19,8 +19,9 @@ in place.
 On CUDA the work runs in this package's sm_100a kernels (``csrc/bssm_conv.cu``,
 ``csrc/bssm_selective.cu``) on the current stream, with gradients for every
 input of :func:`causal_conv` and :func:`selective_scan`; sums and states are
-float32 whatever the rows' type, and results do not differ from run to run.  On
-CPU tensors the same formulas run as PyTorch operations.
+float32 whatever the rows' type, and results do not differ from run to run.
+Forward-mode derivatives are refused.  On CPU tensors the same formulas run as
+PyTorch operations.
 """
 from __future__ import annotations
 
@@ -30,6 +31,7 @@ from typing import Optional, Sequence
 import torch
 import torch.nn.functional as F
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _capi
@@ -120,6 +122,14 @@ def _gradients_wanted(*tensors) -> bool:
             if x is not None and x.requires_grad:
                 return True
     return False
+
+
+def _carries_tangent(*tensors) -> bool:
+    """Whether a tensor is a dual one, of forward-mode differentiation (which no grad mode turns off).  The kernels
+    have none: the autograd functions raise on such a tensor, where the bare calls would drop its tangent."""
+    if forward_ad._current_level < 0:
+        return False
+    return any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors)
 
 
 # ---------------------------------------------------------------------------
@@ -248,7 +258,7 @@ def causal_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, *, act
         return causal_conv_torch(x, weight, bias, activation=activation, initial_state=initial_state,
                                  sequences=sequences)
     silu = int(activation == "silu")
-    if _gradients_wanted(x, weight, bias, initial_state):
+    if _gradients_wanted(x, weight, bias, initial_state) or _carries_tangent(x, weight, bias, initial_state):
         return _CausalConv.apply(x, weight, bias, initial_state, silu, count, tokens, sequences)
     return _conv_forward(x, weight, bias, silu, initial_state, count, tokens, offsets)
 
@@ -271,6 +281,8 @@ def causal_conv_step(x: Tensor, state: Tensor, weight: Tensor, bias: Optional[Te
         y, final = causal_conv_torch(x[:, None], weight, bias, activation=activation, initial_state=state)
         state.copy_(final)
         return y[:, 0]
+    if _carries_tangent(x, weight, bias, state):
+        raise RuntimeError("causal_conv_step has no gradient, in forward mode either: call causal_conv")
     if not state.is_contiguous():
         raise ValueError("state must be contiguous: it is moved on in place")
     x, stride = _rows(x, 1)
@@ -475,7 +487,7 @@ def selective_scan(values: Tensor, steps: Tensor, rates: Tensor, keys: Tensor, q
     if initial_state is not None:
         initial_state = initial_state.float()
     args = (values, steps, rates, keys, queries, skip, gate, step_bias, initial_state)
-    if _gradients_wanted(*args):
+    if _gradients_wanted(*args) or _carries_tangent(*args):
         return _SelectiveScan.apply(*args, groups, int(softplus), count, tokens, longest, sequences)
     return _scan_forward(*args, groups, int(softplus), count, tokens, longest, offsets, False)[:2]
 
@@ -506,6 +518,8 @@ def selective_step(values: Tensor, steps: Tensor, rates: Tensor, keys: Tensor, q
                                            initial_state=state)
         state.copy_(final)
         return read[:, 0]
+    if _carries_tangent(values, steps, rates, keys, queries, state, skip, gate, step_bias):
+        raise RuntimeError("selective_step has no gradient, in forward mode either: call selective_scan")
     if state.dtype != torch.float32 or not state.is_contiguous():
         raise ValueError("state must be float32 and contiguous: it is moved on in place")
     kept, flat = _scan_rows(values, steps, keys, queries, gate)

@@ -13,6 +13,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import plain_selective as plain
 from bayes_ssm.distill import distillation_loss, distillation_loss_torch
@@ -321,3 +322,18 @@ def test_teacher_without_a_distribution(rows, vocab, value):
         second = torch.autograd.grad(loss, x)[0]
         for grad in (first, second):
             assert torch.isnan(grad[1]).all() and torch.isfinite(grad[0]).all() and torch.isfinite(grad[2:]).all()
+
+
+def test_forward_mode_is_refused():
+    """A tangent of the logits must not be lost without a word; the teacher is taken as a constant, as on the CPU."""
+    logits, teacher, indices = inputs(3, 50, 4, torch.float32, 26)
+    want = distillation_loss(logits, teacher, indices)
+    with forward_ad.dual_level():
+        for keep in (True, False):
+            with torch.set_grad_enabled(keep), pytest.raises(NotImplementedError, match="forward mode AD"):
+                distillation_loss(forward_ad.make_dual(logits, torch.ones_like(logits)), teacher, indices)
+        assert torch.equal(distillation_loss(logits, teacher, indices), want)
+        dual = forward_ad.make_dual(teacher, torch.ones_like(teacher))
+        for device in ("cuda", "cpu"):
+            loss = distillation_loss(logits.to(device), dual.to(device), indices.to(device))
+            assert forward_ad.unpack_dual(loss).tangent is None

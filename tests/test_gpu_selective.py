@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import plain_selective as plain
 from bayes_ssm.selective import (PackedSequences, causal_conv, causal_conv_step, selective_scan, selective_step)
@@ -474,3 +475,34 @@ def test_growing_states_that_are_still_zero(shape, n):
     gy[:, 20:] = 0
     want = torch.autograd.grad(call_plain(r, False, None)[0], r["values"], gy.double())[0]
     close(torch.autograd.grad(call(k, False, None)[0], k["values"], gy)[0], want, 2e-5, "grad values")
+
+
+def test_forward_mode_is_refused():
+    """A tangent that came in must not be lost without a word."""
+    i, _ = scan_inputs((2, 9), 16, 8, 1, torch.float32, 41)
+    x, w, b, s, _ = conv_inputs((2, 9), 16, 4, torch.float32, 42)
+    conv = dict(x=x, weight=w, bias=b, initial_state=s)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        for keep in (True, False):
+            with torch.set_grad_enabled(keep):
+                for name in NAMES:
+                    with pytest.raises(NotImplementedError, match="forward mode AD"):
+                        call(dict(i, **{name: dual(i[name])}), True, None)
+                for name in conv:
+                    with pytest.raises(NotImplementedError, match="forward mode AD"):
+                        causal_conv(**dict(conv, **{name: dual(conv[name])}))
+                for name in ("x", "weight", "bias"):
+                    one = dict(x=x[:, 0], weight=w, bias=b)
+                    with pytest.raises(RuntimeError, match="no gradient"):
+                        causal_conv_step(state=s.clone(), **dict(one, **{name: dual(one[name])}))
+                for name in NAMES:
+                    one = {n: v[:, 0] if n in ("values", "steps", "keys", "queries", "gate") else v.clone()
+                           for n, v in i.items()}
+                    one[name] = dual(one[name])
+                    with pytest.raises(RuntimeError, match="no gradient"):
+                        selective_step(*(one[n] for n in NAMES[:5]), one["state"], skip=one["skip"], gate=one["gate"],
+                                       step_bias=one["step_bias"], softplus=True)
+        call(i, True, None)
+        causal_conv(**conv)
