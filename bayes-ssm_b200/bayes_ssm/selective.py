@@ -132,6 +132,12 @@ def _carries_tangent(*tensors) -> bool:
     return any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors)
 
 
+def _written(x: Tensor) -> None:
+    """Tells autograd that a kernel wrote ``x``: a backward that saved it must not read it any more."""
+    if not x.is_inference():  # has no version to count
+        torch.autograd.graph.increment_version(x)
+
+
 # ---------------------------------------------------------------------------
 # Causal convolution
 # ---------------------------------------------------------------------------
@@ -293,6 +299,7 @@ def causal_conv_step(x: Tensor, state: Tensor, weight: Tensor, bias: Optional[Te
                  weight.shape[1], weight.data_ptr(), _DTYPES[weight.dtype], _capi.ptr(bias),
                  0 if bias is None else _DTYPES[bias.dtype], int(activation == "silu"), state.data_ptr(),
                  y.data_ptr())
+    _written(state)
     return y
 
 
@@ -530,6 +537,7 @@ def selective_step(values: Tensor, steps: Tensor, rates: Tensor, keys: Tensor, q
     _capi.launch(values.device, "bssm_selective_step", *flat, _DTYPES[values.dtype], rates.data_ptr(),
                  _capi.ptr(skip), _capi.ptr(step_bias), int(softplus), b, channels, n, groups, state.data_ptr(),
                  out.data_ptr())
+    _written(state)
     del kept
     return out
 

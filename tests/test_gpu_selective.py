@@ -506,3 +506,30 @@ def test_forward_mode_is_refused():
                                        step_bias=one["step_bias"], softplus=True)
         call(i, True, None)
         causal_conv(**conv)
+
+
+def test_steps_in_place_are_seen_by_autograd():
+    """A backward that still needs the state a step has moved on says so instead of using the moved one."""
+    x, w, b, s, _ = conv_inputs((2, 9), 16, 4, torch.float32, 43)
+    wk = w.detach().requires_grad_()
+    y, _ = causal_conv(x, wk, b, activation="silu", initial_state=s)
+    causal_conv_step(x[:, 0], s, w, b, activation="silu")
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    i, _ = scan_inputs((2, 9), 16, 8, 1, torch.float32, 44)
+    scale = torch.ones((), device="cuda", requires_grad=True)
+    used = i["state"] * scale  # keeps the state for its backward
+    head = {n: v[:, 0] if n in ("values", "steps", "keys", "queries", "gate") else v for n, v in i.items()}
+    selective_step(*(head[n] for n in NAMES[:5]), i["state"], skip=head["skip"], gate=head["gate"],
+                   step_bias=head["step_bias"], softplus=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        used.sum().backward()
+    with torch.inference_mode():  # states without a version are moved on all the same
+        y, state = causal_conv(x, w, b)
+        _, hidden = call(i, True, None)
+        causal_conv_step(x[:, 0], state, w, b)
+    kept = state.clone(), hidden.clone()
+    with torch.no_grad():
+        causal_conv_step(x[:, 0], state, w, b)
+        selective_step(*(head[n] for n in NAMES[:5]), hidden, softplus=True)
+    assert not torch.equal(state, kept[0]) and not torch.equal(hidden, kept[1])
