@@ -72,15 +72,17 @@ def _forward(logits, teacher, indices, temperature, reduction, with_grad):
 class _Distillation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, teacher, indices, temperature, reduction):
-        loss, ctx.grad, scratch = _forward(logits, teacher, indices, temperature, reduction, True)
-        ctx.save_for_backward(logits, teacher, indices, scratch)
+        # the gradient is saved with the rest, so that recomputation and offloading take it along
+        loss, grad, scratch = _forward(logits, teacher, indices, temperature, reduction, True)
+        ctx.save_for_backward(logits, teacher, indices, scratch, grad)
+        ctx.unused = grad is not None
         ctx.settings = (temperature, reduction)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, upstream):
-        logits, teacher, indices, scratch = ctx.saved_tensors
+        logits, teacher, indices, scratch, grad = ctx.saved_tensors
         temperature, reduction = ctx.settings
         dev = logits.device
         upstream = upstream.float().contiguous()
@@ -93,8 +95,9 @@ class _Distillation(torch.autograd.Function):
                 reduction == "mean", at, at + 12 * rows, upstream.data_ptr())
         # The gradient written by the forward is handed out once, as it is where the upstream one is 1 and computed
         # again where not (the factor comes before the rounding); a second walk through a retained graph makes its own.
-        grad, ctx.grad = ctx.grad, None
-        if grad is not None:
+        if ctx.unused:
+            ctx.unused = False
+            grad = grad.data  # with a version of its own: its owner may change it while the graph is retained
             _capi.launch(dev, "bssm_distillation_rescale", *flat, grad.data_ptr())
         else:
             grad = _empty_like(logits)

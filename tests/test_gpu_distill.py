@@ -9,10 +9,12 @@ spacing.
 """
 from __future__ import annotations
 
+import gc
 import math
 
 import pytest
 import torch
+import torch.utils.checkpoint
 from torch.autograd import forward_ad
 
 import plain_selective as plain
@@ -337,3 +339,41 @@ def test_forward_mode_is_refused():
         for device in ("cuda", "cpu"):
             loss = distillation_loss(logits.to(device), dual.to(device), indices.to(device))
             assert forward_ad.unpack_dual(loss).tangent is None
+
+
+def test_nothing_of_the_logits_size_is_kept_past_the_hooks():
+    """Recomputation and offloading of what a graph saves reach the gradient that the forward wrote."""
+    g = torch.Generator(device="cuda").manual_seed(24)
+    h = torch.randn(512, 64, generator=g, device="cuda").requires_grad_()
+    w = (torch.randn(20000, 64, generator=g, device="cuda") * 0.3).requires_grad_()
+    teacher, indices = torch.topk(torch.randn(512, 20000, generator=g, device="cuda"), 8, -1)
+
+    def head(a, b):
+        return distillation_loss(a @ b.t(), teacher, indices)
+    want = torch.autograd.grad(head(h, w), (h, w))
+    size = 512 * 20000 * 4
+    for way in ("recomputed", "offloaded"):
+        gc.collect()
+        before = torch.cuda.memory_allocated()
+        if way == "recomputed":
+            loss = torch.utils.checkpoint.checkpoint(head, h, w, use_reentrant=False)
+        else:
+            with torch.autograd.graph.save_on_cpu():
+                loss = head(h, w)
+        assert torch.cuda.memory_allocated() - before < size // 4, way
+        got = torch.autograd.grad(loss * 2.0, (h, w))
+        assert all(rel(a, 2.0 * b) <= 1e-5 for a, b in zip(got, want)), way
+
+
+def test_a_gradient_changed_in_place_between_two_walks():
+    logits, teacher, indices = inputs(5, 200, 4, torch.float32, 25)
+    x = logits.requires_grad_()
+    loss = distillation_loss(x, teacher, indices)
+    want = torch.autograd.grad(distillation_loss(x, teacher, indices), x)[0]
+    loss.backward(retain_graph=True)
+    x.grad.mul_(0.25)
+    loss.backward(retain_graph=True)
+    assert rel(x.grad, 1.25 * want) <= 1e-6
+    x.grad.zero_()
+    loss.backward()
+    assert rel(x.grad, want) <= 1e-6
