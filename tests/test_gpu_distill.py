@@ -377,3 +377,26 @@ def test_a_gradient_changed_in_place_between_two_walks():
     x.grad.zero_()
     loss.backward()
     assert rel(x.grad, want) <= 1e-6
+
+
+# a stretch too long for the bitmap of named entries; rows over 8 CTAs whose doubled entries lie in the first stretch, in
+# the last one and on both sides of a boundary (6,252 float32, 6,256 bfloat16 logits)
+@pytest.mark.parametrize("dtype,rows,vocab", [(torch.float32, 2, 400003), (torch.float32, 3, 50001),
+                                              (torch.bfloat16, 3, 50001), (torch.bfloat16, 1, 800000)])
+def test_doubled_entries_over_several_ctas(rows, vocab, dtype):
+    logits, _, _ = inputs(rows, vocab, 4, dtype, 27)
+    named = [0, 0, 5, 6251, 6252, 6251, 6252, 6255, 6256, 6256, 12503, 12504, 12504, 12512, 12511, vocab - 1, vocab - 1,
+             vocab - 2, 7, -1]
+    indices = torch.tensor(named, device="cuda").repeat(rows, 1)
+    g = torch.Generator(device="cuda").manual_seed(28)
+    teacher = torch.randn(rows, len(named), generator=g, device="cuda")
+    want, x64 = reference(logits, teacher, indices, 1.0, "sum")
+    x = logits.requires_grad_()
+    loss = distillation_loss(x, teacher, indices, reduction="sum")
+    assert abs(float(loss.detach()) - float(want.detach())) <= 1e-5 * (rows + abs(float(want.detach())))
+    ref = torch.autograd.grad(want, x64)[0]
+    for keep in (True, False):  # written by the forward, then from the rows' statistics
+        got = torch.autograd.grad(loss, x, retain_graph=keep)[0]
+        assert rel(got, ref) <= TOL[dtype]
+        at = indices[0, :-1]
+        assert rel(got[:, at], ref[:, at]) <= TOL[dtype]

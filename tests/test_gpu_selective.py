@@ -533,3 +533,77 @@ def test_steps_in_place_are_seen_by_autograd():
         causal_conv_step(x[:, 0], state, w, b)
         selective_step(*(head[n] for n in NAMES[:5]), hidden, softplus=True)
     assert not torch.equal(state, kept[0]) and not torch.equal(hidden, kept[1])
+
+
+# ---------------------------------------------------------------------------
+# sizes that the small cases above do not reach
+# ---------------------------------------------------------------------------
+
+def conv_wide(x, weight, bias, silu, state, lengths):
+    """The plain form of a convolution, all tokens at a time."""
+    taps, ys, finals = weight.shape[1], [], []
+    for r, past in zip(plain.runs(x, lengths), state):
+        wide = torch.cat([past, r])
+        u = sum(wide[j:j + r.shape[0]] * weight[:, j] for j in range(taps)) + bias
+        ys.append(u * torch.sigmoid(u) if silu else u)
+        finals.append(wide[r.shape[0]:])
+    return (torch.stack(ys) if lengths is None else torch.cat(ys)), torch.stack(finals)
+
+
+# a thread's run of tokens grows from 4 with the number of elements: 8 (2.7 million), 32 (10 and 11) and, backward, 64
+# (20), over odd and even channel counts
+@pytest.mark.parametrize("shape,c,taps,dtype", [
+    ((7, 391), 1001, 3, torch.bfloat16), ((5, 521), 4000, 4, torch.bfloat16), ((3, 1663), 4002, 2, torch.float32),
+    ((5, 521), 4000, 3, torch.float32), ([0, 700, 1, 37, 2000, 0, 3], 4001, 3, torch.float16),
+    ([0, 700, 1, 37, 2000, 0, 3], 4000, 4, torch.float32), ((2, 2500), 4001, 4, torch.bfloat16)])
+def test_conv_long_runs(shape, c, taps, dtype):
+    x, w, b, s, lengths = conv_inputs(shape, c, taps, dtype, 51, wdtype=torch.float32)
+    seqs = None if lengths is None else PackedSequences(lengths, device="cuda")
+    r, k = leaves64(x, w, b, s), leaves(x, w, b, s)
+    want = conv_wide(*r[:3], True, r[3], lengths)
+    outs = causal_conv(k[0], k[1], k[2], activation="silu", initial_state=k[3], sequences=seqs)
+    close(outs[0], want[0], TOL[dtype], "y")
+    assert torch.equal(outs[1].detach().double(), want[1].detach())
+    assert torch.equal(causal_conv(x, w, b, activation="silu", initial_state=s, sequences=seqs)[0], outs[0].detach())
+    g = gen(52)
+    ups = [rand(g, *o.shape, dtype=dtype) for o in outs]
+    got = torch.autograd.grad(outs, k, ups)
+    ref = torch.autograd.grad(want, r, [u.double() for u in ups])
+    for name, a, v in zip(("x", "weight", "bias", "state"), got, ref):
+        close(a, v, TOL[a.dtype], f"grad {name}")
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("b,c,n,groups", [(1500, 40, 16, 1), (200, 300, 10, 3), (400, 64, 64, 2), (700, 300, 1, 1),
+                                          (1300, 17, 4, 1)])
+def test_steps_of_many_sequences(b, c, n, groups, dtype):
+    """More sequences than one wave of CTAs takes: a lane walks several of them."""
+    i, _ = scan_inputs((b, 1), c, n, groups, dtype, 53)
+    want, want_final = call_plain({name: v.double() for name, v in i.items()}, True, None)
+    one = {name: v[:, 0] if name in ("values", "steps", "keys", "queries", "gate") else v for name, v in i.items()}
+    got = selective_step(*(one[name] for name in NAMES[:5]), one["state"], skip=one["skip"], gate=one["gate"],
+                         step_bias=one["step_bias"], softplus=True)
+    close(got[:, None], want, TOL[dtype], "read")
+    close(one["state"], want_final, TOL[torch.float32], "state")
+    assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16))
+@pytest.mark.parametrize("shape,c,n,groups", [((2, 70), 300, 1, 1), ((1, 90), 512, 2, 2), ((2, 48), 256, 2, 1),
+                                              ([33, 0, 1, 100], 257, 1, 1), ((1, 800), 20, 2, 1)])
+def test_scan_of_one_and_two_states(shape, c, n, groups, dtype):
+    """A lane to a channel, over several tiles and segments, with and without channels left over."""
+    i, lengths = scan_inputs(shape, c, n, groups, dtype, 54)
+    seqs = None if lengths is None else PackedSequences(lengths, device="cuda")
+    r = dict(zip(NAMES, leaves64(*(i[k] for k in NAMES))))
+    k = dict(zip(NAMES, leaves(*(i[k] for k in NAMES))))
+    want, want_final = call_plain(r, True, lengths)
+    y, final = call(k, True, seqs)
+    close(y, want, TOL[dtype], "read")
+    close(final, want_final, 2e-5, "state")
+    g = gen(55)
+    gy, gf = rand(g, *y.shape, dtype=dtype), rand(g, *final.shape)
+    got = torch.autograd.grad((y, final), [k[name] for name in NAMES], (gy, gf))
+    ref = torch.autograd.grad((want, want_final), [r[name] for name in NAMES], (gy.double(), gf.double()))
+    for name, a, b in zip(NAMES, got, ref):
+        close(a, b, TOL[a.dtype], f"grad {name}")
