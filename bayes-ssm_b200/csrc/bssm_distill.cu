@@ -16,9 +16,10 @@
 // once.  A CTA takes a row (where rows are few, a cluster of CTAs takes one,
 // each a stretch of the vocabulary): a pass for the running reference and sum,
 // and, where the gradient is wanted, a second one over logits that are then in
-// L2 (4 rows an SM of 64 to 128 KB are 38 to 76 MB of its 126).  The K entries
-// are corrected afterwards, from the logits again rather than from the rounded
-// gradient.  Sums are float32, taken in an order that sizes alone decide.
+// L2 (6 CTAs an SM with stretches of up to 80 KB are 71 of its 126 MB; a row of
+// more than 8 such stretches has longer ones, which may outgrow it).  The K
+// entries are corrected afterwards, from the logits again rather than from the
+// rounded gradient.  Sums are float32, taken in an order that sizes alone decide.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -175,7 +176,7 @@ template <typename T, bool BACKWARD, int THREADS>
 __device__ __forceinline__ void distill_row(const DistillArgs &a, const long r) {
     constexpr int kVec = 16 / sizeof(T), kWarps = THREADS / 32;
     __shared__ float p_s[kMaxTop];
-    __shared__ __align__(16) int i_s[kMaxTop + 4];
+    __shared__ int i_s[kMaxTop];
     __shared__ float2 stat_s[kWarps], teacher_s[kWarps];
     __shared__ float loss_s[kWarps];
     __shared__ int bad_s[kWarps], count_s[kWarps], again_s;
@@ -208,7 +209,6 @@ __device__ __forceinline__ void distill_row(const DistillArgs &a, const long r) 
         bad |= j == -2;
         top = fmaxf(top, j == -1 ? -INFINITY : t);
     }
-    if (tid < 4) i_s[a.top + tid] = -1;
     const bool any = __any_sync(0xffffffffu, top != -INFINITY);
     bool nan = false;  // a NaN gives way in fmaxf, but is an entry
     for (int k = tid; k < a.top; k += THREADS) nan |= p_s[k] != p_s[k];
@@ -452,7 +452,7 @@ template <typename T> int launch_rows(DistillArgs a, RowsKind kind, cudaStream_t
     config.numAttrs = ranks > 1 ? 1 : 0;  // a cluster of one costs: 65,536 x 256 bf16 289 us with it, 159 without
     // Short rows are bound by a row's chain of round trips, so more of them at a time, by fewer threads each.  64, 128
     // and 256 threads: 65,536 x 256 bf16 159, 244, 452 us; 32,768 x 4,096 bf16 159, 196, 318; 32,768 x 4,096 f32 249,
-    // 239, 321; 8,192 x 16,000 bf16 177, 118, 142; 8,192 x 32,000 bf16 (12 rows an SM are then more than L2) -, 258, 204.
+    // 239, 321; 8,192 x 16,000 bf16 177, 118, 142; 8,192 x 32,000 bf16 -, 258 (12 rows an SM are more than L2), 204.
     const long bytes = static_cast<long>(a.vocab) * static_cast<long>(sizeof(T));
     const unsigned split = static_cast<unsigned>(ranks);
     const cudaError_t e = ranks > 1 || bytes > 32768 ? launch_kernel<T, 256>(config, split, a, kind)

@@ -39,11 +39,14 @@ __device__ __forceinline__ void store_from_float(void *p, int dtype, long i, flo
 __host__ __device__ constexpr bool io_dtype_known(int dtype) {
     return dtype == BSSM_F32 || dtype == BSSM_BF16 || dtype == BSSM_F16;
 }
-__host__ __device__ constexpr int io_dtype_bytes(int dtype) { return dtype == BSSM_F32 ? 4 : 2; }
 
 // VEC consecutive elements as float32, in one access when VEC * sizeof(T) <= 16
 // (the address must then be a multiple of that), else in 16-byte accesses.
-template <typename T, int VEC> struct alignas((VEC & (VEC - 1)) != 0 ? sizeof(T) : VEC * sizeof(T) < 16 ? VEC * sizeof(T) : 16) Packed {
+template <typename T, int VEC> constexpr int packed_alignment() {
+    constexpr int bytes = VEC * static_cast<int>(sizeof(T));
+    return (VEC & (VEC - 1)) != 0 ? static_cast<int>(sizeof(T)) : bytes < 16 ? bytes : 16;
+}
+template <typename T, int VEC> struct alignas(packed_alignment<T, VEC>()) Packed {
     T e[VEC];
 };
 template <typename T, int VEC> __device__ __forceinline__ void widen(const Packed<T, VEC> &p, float (&o)[VEC]) {
@@ -88,7 +91,10 @@ template <typename T, int VEC> struct RawVec {
         if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
         else if constexpr (std::is_same<T, __nv_bfloat16>::value)
             return __uint_as_float(i % 2 == 0 ? w[i / 2] << 16 : w[i / 2] & 0xffff0000u);
-        else return __half2float(__ushort_as_half(static_cast<unsigned short>(i % 2 == 0 ? w[i / 2] & 0xffffu : w[i / 2] >> 16)));
+        else {
+            const unsigned bits = i % 2 == 0 ? w[i / 2] & 0xffffu : w[i / 2] >> 16;
+            return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+        }
     }
     __device__ __forceinline__ void values(float (&o)[VEC]) const {
 #pragma unroll

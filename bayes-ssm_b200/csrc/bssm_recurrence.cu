@@ -944,7 +944,7 @@ const char *bssm_last_error(void) { return g_last_error.c_str(); }
 
 int bssm_debug_last_family(void) { return bssm::g_last_family; }
 
-int bssm_version(void) { return 10101; }
+int bssm_version(void) { return 10200; }
 
 int bssm_forward_chunked_ex(int key_dim, int value_dim, int io_dtype, int fixed, const void *keys,
                             const void *values, const void *queries, const float *decay,

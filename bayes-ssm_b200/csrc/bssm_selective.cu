@@ -916,7 +916,7 @@ template <typename T, int VEC> struct StepKeys {  // VEC adjacent keys on their 
     unsigned w[VEC];
     __device__ __forceinline__ void load(const T *p, int n, bool wide) {
         if (sizeof(T) == 2 && VEC > 1 && wide) {
-            const Packed<unsigned, (VEC + 1) / 2> v = load_packed<unsigned, (VEC + 1) / 2>(reinterpret_cast<const unsigned *>(p));
+            const auto v = load_packed<unsigned, (VEC + 1) / 2>(reinterpret_cast<const unsigned *>(p));
 #pragma unroll
             for (int j = 0; j < (VEC + 1) / 2; ++j) w[j] = v.e[j];
         } else {

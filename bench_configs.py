@@ -624,7 +624,8 @@ def selective(steps: int, warmup: int) -> dict:
     return {"config": "selective", "metric": "tok/s", "value": round(b * t / train_ms * 1e3, 1), "unit": "tok/s",
             "train_ms": round(train_ms, 3), "train_kernels_ms": round(own_ms(train), 3),
             "prefill_ms": round(prefill_ms, 3), "prefill_kernels_ms": round(own_ms(lambda: model.prefill(tokens)), 3),
-            "step_us": round(step_ms * 1e3, 1), "step_graph_us": round(graph_ms * 1e3, 1), "step_kernels_us": round(own_ms(lambda: model.step(one, state)) * 1e3, 1),
+            "step_us": round(step_ms * 1e3, 1), "step_graph_us": round(graph_ms * 1e3, 1),
+            "step_kernels_us": round(own_ms(lambda: model.step(one, state)) * 1e3, 1),
             "parameters": parameter_count(model), "batch": b, "tokens": t, "loss": float(train()), "data": "synthetic"}
 
 
